@@ -1,0 +1,216 @@
+// Kernel arguments of the paged-cache operators' module (paged_ops.cubin),
+// shared by the device code and the host library. Every kernel takes one of
+// these structs by value; the host launches them through lr_launch* with the
+// struct as the packed argument blob. The operators are described in
+// include/lrrt_ops.h.
+#ifndef LRRT_OPS_KERNELS_HPP_
+#define LRRT_OPS_KERNELS_HPP_
+
+#include <cstdint>
+
+#if defined(__CUDACC__)
+#define LRRT_OPS_HD __host__ __device__
+#else
+#define LRRT_OPS_HD
+#endif
+
+namespace lrrt::ops {
+
+// n / divisor for n < 2^31 as one multiplication: with 2^(s-1) < d <= 2^s and
+// m = ceil(2^(31+s) / d) < 2^32, n m = 2^(31+s) n / d + n e / d with e < d, and
+// the excess n e / (d 2^(31+s)) < 2^-s <= 1 / d never reaches the next integer.
+struct Divider {
+  uint32_t divisor, multiplier, shift; // shift = s - 1; divisor 1 has none
+
+  static Divider of(uint32_t d) {
+    uint32_t s = 0;
+    while ((uint64_t{1} << s) < d) {
+      ++s;
+    }
+    const uint64_t m = ((uint64_t{1} << (31u + s)) + d - 1u) / d;
+    return {d, static_cast<uint32_t>(m), s == 0 ? 0u : s - 1u};
+  }
+  LRRT_OPS_HD uint32_t quotient(uint32_t n) const {
+    if (divisor == 1) {
+      return n;
+    }
+#if defined(__CUDA_ARCH__)
+    return __umulhi(n, multiplier) >> shift;
+#else
+    return static_cast<uint32_t>((uint64_t{n} * multiplier) >> 32) >> shift;
+#endif
+  }
+};
+
+struct Rows {
+  void *data;
+  int64_t row_stride, head_stride; // elements
+};
+
+struct Cache {
+  void *keys, *values;
+  int64_t key_page, key_token, key_head; // strides, elements
+  int64_t value_page, value_token, value_head;
+  uint32_t page_count, kv_heads;
+  Divider page;
+};
+
+struct Table {
+  const int32_t *pages;
+  int64_t row_stride;
+  uint32_t rows, columns;
+};
+
+constexpr uint32_t kRopeThreads = 256;
+
+struct RopeAppendArgs {
+  Rows q, q_out, k, v;
+  Cache cache;
+  Table table;
+  const int32_t *sequences, *positions;
+  const float *cos_table, *sin_table;
+  uint64_t items; // tokens * items_per_token
+  uint32_t heads, head_dim, rotary_dim, table_positions;
+  // One item is a vector of `width` elements of a head that is copied, or a
+  // vector of each half of its pairs that is rotated.
+  uint32_t items_per_token, turned_items; // turned: those of the q and k heads
+  Divider per_token, per_head, per_value_head;
+};
+
+// Shared memory of an attention block: a ring of kAttentionStages tiles for
+// each of its warps. A tile is 16 keys and values, or 32 of the short rows of
+// 128 bytes: 8 KB, and 16 KB for rows of 512 bytes; eight warps, or four.
+constexpr uint32_t kAttentionStages = 3;
+constexpr uint32_t kAttentionRingBytes = 196608;
+// Tiles that a block takes at least, so that a short row is not split into
+// more partial states than its tiles are worth.
+constexpr uint32_t kAttentionMinimumTiles = 16;
+
+LRRT_OPS_HD constexpr uint32_t attention_tile_bytes(uint32_t row_bytes) {
+  return row_bytes <= 256u ? 8192u : 16384u;
+}
+LRRT_OPS_HD constexpr uint32_t attention_tile_keys(uint32_t row_bytes) {
+  return attention_tile_bytes(row_bytes) / (2u * row_bytes);
+}
+LRRT_OPS_HD constexpr uint32_t attention_warps(uint32_t row_bytes) {
+  return kAttentionRingBytes / (kAttentionStages * attention_tile_bytes(row_bytes));
+}
+// The blocks' merge area: one state of 8 heads per warp, and at least the
+// join's weights of every block for 16 heads.
+LRRT_OPS_HD constexpr uint32_t attention_merge_floats(uint32_t dim, uint32_t row_bytes) {
+  const uint32_t states = attention_warps(row_bytes) * 8u * dim;
+  return states < 4096u ? 4096u : states;
+}
+LRRT_OPS_HD constexpr uint32_t attention_shared_bytes(uint32_t dim, uint32_t row_bytes) {
+  return kAttentionRingBytes + 4u * attention_merge_floats(dim, row_bytes) + 2048u;
+}
+// One partial state: the weighted values, the maxima and the sums of a
+// block's heads.
+LRRT_OPS_HD constexpr uint32_t attention_state_floats(uint32_t dim, uint32_t heads) {
+  return heads * (dim + 2u);
+}
+
+struct PagedAttentionArgs {
+  Rows q, out;
+  Cache cache;
+  Table table;
+  const int32_t *lengths;
+  const float *slopes; // null: no distance bias
+  float *lse;          // null: not wanted
+  float *states;       // [2 * grid][attention_state_floats]
+  uint32_t *arrivals;  // [table.rows * rows_per_sequence], zero between launches
+  uint32_t heads, group, head_dim, window;
+  uint32_t head_blocks, rows_per_sequence; // blocks of query heads per kv head; kv_heads * them
+  float scale, softcap;
+};
+
+// One run of pages: `rows` rows of page `source` go to page `target`.
+struct PageMove {
+  int32_t source, target;
+  uint32_t rows, reserved;
+};
+
+constexpr uint32_t kPlanBlocks = 8; // one cluster
+constexpr uint32_t kPlanThreads = 512;
+
+struct ForkArgs {
+  Table table;
+  const int32_t *lengths, *parents;
+  const uint8_t *held;
+  int32_t *table_out;
+  int64_t table_out_stride;
+  int32_t *lengths_out, *status;
+  uint32_t rows_out, room, page_count;
+  Divider page;
+  uint32_t *owners;    // [page_count]
+  int32_t *free_pages; // [page_count]
+  uint32_t *first_new; // [rows_out]
+  uint32_t *first_copy; // [rows_out]
+  PageMove *moves;     // [rows_out]
+  uint32_t *move_count;
+};
+
+struct CompactArgs {
+  Table table;
+  const uint8_t *held;
+  int32_t *table_out;
+  int64_t table_out_stride;
+  int32_t *status;
+  uint32_t page_count, page_size;
+  uint32_t *marks;     // [page_count]
+  int32_t *free_pages; // [page_count]
+  uint32_t *ranks;     // [page_count]
+  PageMove *moves;     // [page_count]
+  uint32_t *move_count;
+};
+
+constexpr uint32_t kMoveThreads = 256;
+constexpr uint32_t kMoveSliceVectors = 256; // vectors of one warp's slice: eight per lane
+
+struct MoveArgs {
+  void *keys, *values;
+  int64_t layer_stride, page_stride; // bytes
+  const PageMove *moves;             // null: sources and targets, whole pages
+  const uint32_t *move_count;
+  const int32_t *sources, *targets;
+  uint32_t count; // without move_count
+  uint32_t page_count, page_size, segments, row_bytes;
+  uint32_t units_per_move; // layers * 2 * segments * slices
+  Divider per_move, per_segment; // units of a move; slices of a segment
+  Divider segments_divider;
+};
+
+constexpr uint32_t kBeamThreads = 256;
+constexpr uint32_t kBeamMaximumCount = 64;
+constexpr uint32_t kBeamMaximumCandidates = 2048; // beams * count
+
+struct Pair {
+  float x, y;
+};
+
+struct BeamArgs {
+  const void *logits;
+  int64_t logits_stride;
+  const float *scores;
+  const uint8_t *finished;
+  float *scores_out;
+  int32_t *parents_out, *tokens_out;
+  uint8_t *finished_out;
+  uint32_t groups, beams, vocab, count, chunks;
+  int32_t end_token;
+  uint64_t *chunk_keys;   // [rows][chunks][count]
+  Pair *chunk_sums;       // [rows][chunks] maximum, sum of exponentials
+  uint64_t *row_keys;     // [rows][count]
+  float *row_log_sums;    // [rows]
+  uint32_t *row_arrivals; // [rows], zero between launches
+  uint32_t *group_arrivals; // [groups], likewise
+};
+
+struct ZeroArgs {
+  uint32_t *words;
+  uint64_t count;
+};
+
+} // namespace lrrt::ops
+
+#endif // LRRT_OPS_KERNELS_HPP_

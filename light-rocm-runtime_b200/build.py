@@ -6,6 +6,8 @@ Outputs (git-ignored, shipped with the working tree):
   lib/qwen_stateful_graph.cubin   sm_100a decode megakernels
   lib/qwen_prefill.cubin          sm_100a prompt prefill kernels
   lib/decoder_ops.cubin + .json   per-operation decode kernels as an lrrt::bundle
+  lib/liblrrt_ops.so              paged-cache operators (include/lrrt_ops.h)
+  lib/paged_ops.cubin             their sm_100a kernels
   _build/tests/stateful_graph_fixture.cubin  sm_100a scheduler fixture kernels (tests)
   _build/tests/*                  C++ host tests (tests/cpp)
 
@@ -85,10 +87,19 @@ def build(verbose: bool = False) -> dict[str, Path]:
               "-lrt", "-ldl", "-lpthread", "-Wl,-rpath,$ORIGIN"], verbose)
     outputs["driver"] = driver
 
-    for name in ("qwen_stateful_graph", "qwen_prefill", "decoder_ops"):
+    # Paged-cache operators (include/lrrt_ops.h).
+    ops = LIB / "liblrrt_ops.so"
+    ops_sources = sorted((csrc / "ops").glob("*.cpp"))
+    if _stale(ops, ops_sources + headers + [runtime]):
+        _run([CXX, *CXXFLAGS, "-shared", "-fvisibility=hidden", *map(str, ops_sources), "-o",
+              str(ops), f"-L{LIB}", "-llrrt", "-Wl,-rpath,$ORIGIN"], verbose)
+    outputs["ops"] = ops
+
+    for name in ("qwen_stateful_graph", "qwen_prefill", "decoder_ops", "paged_ops"):
         source = csrc / "kernels" / f"{name}.cu"
         cubin = LIB / f"{name}.cubin"
-        if _stale(cubin, [source] + headers):
+        parts = sorted((csrc / "kernels" / "paged").glob("*.cuh")) if name == "paged_ops" else []
+        if _stale(cubin, [source] + parts + headers):
             _run([NVCC, *NVCCFLAGS, "-cubin", str(source), "-o", str(cubin)], verbose)
         outputs[name] = cubin
     # Per-operation decode kernels as a bundle: manifest next to its cubin.
@@ -118,9 +129,9 @@ def build(verbose: bool = False) -> dict[str, Path]:
     outputs["bundle_manifest"] = bundle_manifest
     for source in sorted(tests_dir.glob("*.cpp")):
         binary = test_build / source.stem
-        if _stale(binary, [source] + headers + [runtime, driver]):
+        if _stale(binary, [source] + headers + [runtime, driver, ops]):
             _run([CXX, *CXXFLAGS, str(source), "-o", str(binary), f"-L{LIB}", "-llrrt_qwen",
-                  "-llrrt", "-Wl,-rpath,$ORIGIN/../../lib"], verbose)
+                  "-llrrt_ops", "-llrrt", "-Wl,-rpath,$ORIGIN/../../lib"], verbose)
         outputs[f"test:{source.stem}"] = binary
     return outputs
 

@@ -15,6 +15,7 @@
 // The HSA/AQL queue machinery of the reference has no counterpart: CUDA
 // streams, events and cooperative launches replace it.
 #include "driver.hpp"
+#include "lrrt/interop.h"
 #include "lrrt/lrrt.h"
 
 #include <dlfcn.h>
@@ -33,6 +34,7 @@
 struct lr_queue_t {
   uint32_t device;
   CUstream stream;
+  bool wrapped; // the stream belongs to the caller (lr_queue_wrap_stream)
 };
 
 struct lr_event_t {
@@ -409,7 +411,9 @@ void release_device(DeviceState &state) {
   }
   for (auto it = g_queues.begin(); it != g_queues.end();) {
     if (&g_devices[(*it)->device] == &state) {
-      g_driver.cuStreamDestroy_((*it)->stream);
+      if (!(*it)->wrapped) {
+        g_driver.cuStreamDestroy_((*it)->stream);
+      }
       delete *it;
       it = g_queues.erase(it);
     } else {
@@ -658,7 +662,23 @@ LRRT_API lr_status_t lr_queue_create(lr_device_t device, lr_queue_t **queue) {
   CUstream stream = nullptr;
   LR_TRY(cu(g_driver.cuStreamCreate_(&stream, CU_STREAM_NON_BLOCKING),
             "cuStreamCreate"));
-  lr_queue_t *created = new lr_queue_t{device.index, stream};
+  lr_queue_t *created = new lr_queue_t{device.index, stream, false};
+  g_queues.insert(created);
+  *queue = created;
+  return LR_SUCCESS;
+}
+
+LRRT_API lr_status_t lr_queue_wrap_stream(lr_device_t device, void *stream,
+                                          lr_queue_t **queue) {
+  Lock lock(g_mutex);
+  if (!g_initialized) {
+    return LR_ERROR_NOT_INITIALIZED;
+  }
+  if (open_device_state(device.index) == nullptr || queue == nullptr) {
+    return LR_ERROR_INVALID_ARGUMENT;
+  }
+  lr_queue_t *created =
+      new lr_queue_t{device.index, static_cast<CUstream>(stream), true};
   g_queues.insert(created);
   *queue = created;
   return LR_SUCCESS;
@@ -676,7 +696,9 @@ LRRT_API lr_status_t lr_queue_destroy(lr_queue_t *queue) {
   if (state != nullptr) {
     make_current(*state);
     g_driver.cuStreamSynchronize_(queue->stream);
-    g_driver.cuStreamDestroy_(queue->stream);
+    if (!queue->wrapped) {
+      g_driver.cuStreamDestroy_(queue->stream);
+    }
   }
   g_queues.erase(queue);
   delete queue;

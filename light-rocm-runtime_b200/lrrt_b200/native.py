@@ -1,9 +1,10 @@
-"""ctypes declarations of the package's two C ABIs.
+"""ctypes declarations of the package's C ABIs.
 
-liblrrt.so       -- the lr_* runtime ABI (include/lrrt/lrrt.h)
+liblrrt.so       -- the lr_* runtime ABI (include/lrrt/lrrt.h, lrrt/interop.h)
 liblrrt_qwen.so  -- the Qwen decode driver ABI (include/lrrt_qwen.h)
+liblrrt_ops.so   -- the paged-cache operators' ABI (include/lrrt_ops.h)
 
-Both libraries are built in-tree by ``build.py``; loading fails loudly when
+The libraries are built in-tree by ``build.py``; loading fails loudly when
 they are missing, there is no fallback implementation.
 """
 from __future__ import annotations
@@ -15,10 +16,13 @@ PACKAGE = Path(__file__).resolve().parent.parent
 LIB = PACKAGE / "lib"
 RUNTIME_PATH = LIB / "liblrrt.so"
 DRIVER_PATH = LIB / "liblrrt_qwen.so"
+OPS_PATH = LIB / "liblrrt_ops.so"
+OPS_CUBIN = LIB / "paged_ops.cubin"
 QWEN_CUBIN = LIB / "qwen_stateful_graph.cubin"
 PREFILL_CUBIN = LIB / "qwen_prefill.cubin"
 FIXTURE_CUBIN = PACKAGE / "_build" / "tests" / "stateful_graph_fixture.cubin"
 
+i32, i64, f64 = C.c_int32, C.c_int64, C.c_double
 u32, u64, f32, vp, cp, sz = C.c_uint32, C.c_uint64, C.c_float, C.c_void_p, C.c_char_p, C.c_size_t
 
 LR_SUCCESS = 0
@@ -116,6 +120,65 @@ class ModelInfo(C.Structure):
                 ("weight_bytes_per_token", u64)]
 
 
+class OpsRows(C.Structure):
+    _fields_ = [("data", vp), ("row_stride", i64), ("head_stride", i64)]
+
+
+class OpsCache(C.Structure):
+    _fields_ = [("keys", vp), ("values", vp), ("key_page_stride", i64),
+                ("key_token_stride", i64), ("key_head_stride", i64),
+                ("value_page_stride", i64), ("value_token_stride", i64),
+                ("value_head_stride", i64), ("type", u32), ("page_count", u32),
+                ("page_size", u32), ("kv_heads", u32), ("head_dim", u32)]
+
+
+class OpsTable(C.Structure):
+    _fields_ = [("pages", vp), ("row_stride", i64), ("rows", u32), ("columns", u32)]
+
+
+class RopeAppend(C.Structure):
+    _fields_ = [("q", OpsRows), ("q_out", OpsRows), ("k", OpsRows), ("v", OpsRows),
+                ("cache", OpsCache), ("table", OpsTable), ("sequences", vp), ("positions", vp),
+                ("cos_table", vp), ("sin_table", vp), ("tokens", u32), ("heads", u32),
+                ("rotary_dim", u32), ("table_positions", u32), ("interleaved", u32),
+                ("reserved", u32)]
+
+
+class PagedAttention(C.Structure):
+    _fields_ = [("q", OpsRows), ("out", OpsRows), ("cache", OpsCache), ("table", OpsTable),
+                ("lengths", vp), ("slopes", vp), ("lse", vp), ("heads", u32), ("window", u32),
+                ("scale", f32), ("softcap", f32)]
+
+
+class OpsPool(C.Structure):
+    _fields_ = [("keys", vp), ("values", vp), ("layer_stride_bytes", i64),
+                ("page_stride_bytes", i64), ("layers", u32), ("page_count", u32),
+                ("page_size", u32), ("segments", u32), ("row_bytes", u32), ("reserved", u32)]
+
+
+class PagesFork(C.Structure):
+    _fields_ = [("pool", OpsPool), ("table", OpsTable), ("lengths", vp), ("parents", vp),
+                ("held", vp), ("table_out", vp), ("table_out_row_stride", i64),
+                ("lengths_out", vp), ("status", vp), ("rows_out", u32), ("room", u32)]
+
+
+class PagesCompact(C.Structure):
+    _fields_ = [("pool", OpsPool), ("table", OpsTable), ("held", vp), ("table_out", vp),
+                ("table_out_row_stride", i64), ("status", vp)]
+
+
+class PagesCopy(C.Structure):
+    _fields_ = [("pool", OpsPool), ("sources", vp), ("targets", vp), ("count", u32),
+                ("reserved", u32)]
+
+
+class BeamSelect(C.Structure):
+    _fields_ = [("logits", vp), ("logits_row_stride", i64), ("scores", vp), ("finished", vp),
+                ("scores_out", vp), ("parents_out", vp), ("tokens_out", vp),
+                ("finished_out", vp), ("type", u32), ("groups", u32), ("beams", u32),
+                ("vocab", u32), ("count", u32), ("end_token", i32)]
+
+
 P = C.POINTER
 
 # name -> (restype, argtypes)
@@ -161,6 +224,7 @@ RUNTIME_FUNCTIONS = {
     "lr_kernel_max_resident_blocks": (u32, [vp, u32, u32, P(u32)]),
     "lr_queue_native_handle": (u32, [Device, vp, P(vp)]),
     "lr_last_error_detail": (u32, [C.c_char_p, sz]),
+    "lr_queue_wrap_stream": (u32, [Device, vp, P(vp)]),
 }
 
 DRIVER_FUNCTIONS = {
@@ -206,8 +270,23 @@ DRIVER_FUNCTIONS = {
     "lrq_last_error": (cp, []),
 }
 
+OPS_FUNCTIONS = {
+    "lro_context_create": (u32, [Device, vp, vp, sz, P(vp)]),
+    "lro_context_destroy": (u32, [vp]),
+    "lro_context_reserve": (u32, [vp, sz]),
+    "lro_rope_tables": (u32, [u32, u32, f64, f64, f64, f64, f64, P(f32), P(f32)]),
+    "lro_rope_append": (u32, [vp, P(RopeAppend)]),
+    "lro_paged_attention": (u32, [vp, P(PagedAttention)]),
+    "lro_pages_fork": (u32, [vp, P(PagesFork)]),
+    "lro_pages_compact": (u32, [vp, P(PagesCompact)]),
+    "lro_pages_copy": (u32, [vp, P(PagesCopy)]),
+    "lro_beam_select": (u32, [vp, P(BeamSelect)]),
+    "lro_last_error": (cp, []),
+}
+
 _runtime = None
 _driver = None
+_operators = None
 
 
 def _declare(library: C.CDLL, table: dict) -> C.CDLL:
@@ -239,6 +318,17 @@ def driver() -> C.CDLL:
     return _driver
 
 
+def operators() -> C.CDLL:
+    """The paged-cache operators' library."""
+    global _operators
+    if _operators is None:
+        runtime()
+        if not OPS_PATH.exists():
+            raise RuntimeError(f"{OPS_PATH} is missing: run light-rocm-runtime_b200/build.py")
+        _operators = _declare(C.CDLL(str(OPS_PATH)), OPS_FUNCTIONS)
+    return _operators
+
+
 class LrrtError(RuntimeError):
     def __init__(self, status: int, operation: str, detail: str = ""):
         name = runtime().lr_status_string(status).decode()
@@ -253,4 +343,6 @@ def check(status: int, operation: str) -> None:
         detail = buffer.value.decode(errors="replace")
         if operation.startswith("lrq_"):
             detail = driver().lrq_last_error().decode(errors="replace") or detail
+        elif operation.startswith("lro_"):
+            detail = operators().lro_last_error().decode(errors="replace") or detail
         raise LrrtError(status, operation, detail)
