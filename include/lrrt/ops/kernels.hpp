@@ -77,15 +77,11 @@ struct RopeAppendArgs {
   Divider per_token, per_head, per_value_head;
 };
 
-// Shared memory of an attention block: a ring of kAttentionStages tiles for
-// each of its warps. A tile is 16 keys and values, or 32 of the short rows of
-// 128 bytes: 8 KB, and 16 KB for rows of 512 bytes; eight warps, or four.
-constexpr uint32_t kAttentionStages = 3;
-constexpr uint32_t kAttentionRingBytes = 196608;
-// Tiles that a block takes at least, so that a short row is not split into
-// more partial states than its tiles are worth.
-constexpr uint32_t kAttentionMinimumTiles = 16;
-
+// Shared memory of an attention block: a ring of tiles for each of its warps,
+// and a partial state for each. A tile is 16 keys and values, or 32 of the
+// short rows of 128 bytes: 8 KB, and 16 KB for rows of 512 bytes. Eight warps
+// have three tiles each (two beside states of 16 heads), four where tiles are
+// large.
 LRRT_OPS_HD constexpr uint32_t attention_tile_bytes(uint32_t row_bytes) {
   return row_bytes <= 256u ? 8192u : 16384u;
 }
@@ -93,22 +89,37 @@ LRRT_OPS_HD constexpr uint32_t attention_tile_keys(uint32_t row_bytes) {
   return attention_tile_bytes(row_bytes) / (2u * row_bytes);
 }
 LRRT_OPS_HD constexpr uint32_t attention_warps(uint32_t row_bytes) {
-  return kAttentionRingBytes / (kAttentionStages * attention_tile_bytes(row_bytes));
+  return row_bytes <= 256u ? 8u : 4u;
 }
-// The blocks' merge area: one state of 8 heads per warp, and at least the
-// join's weights of every block for 16 heads.
-LRRT_OPS_HD constexpr uint32_t attention_merge_floats(uint32_t dim, uint32_t row_bytes) {
-  const uint32_t states = attention_warps(row_bytes) * 8u * dim;
-  return states < 4096u ? 4096u : states;
+LRRT_OPS_HD constexpr uint32_t attention_stages(uint32_t heads) {
+  return heads > 8u ? 2u : 3u;
 }
-LRRT_OPS_HD constexpr uint32_t attention_shared_bytes(uint32_t dim, uint32_t row_bytes) {
-  return kAttentionRingBytes + 4u * attention_merge_floats(dim, row_bytes) + 2048u;
-}
-// One partial state: the weighted values, the maxima and the sums of a
-// block's heads.
+// One partial state: the weighted values (rows padded against bank conflicts),
+// the maxima and the sums of a block's heads.
 LRRT_OPS_HD constexpr uint32_t attention_state_floats(uint32_t dim, uint32_t heads) {
-  return heads * (dim + 2u);
+  return heads * (dim + 6u);
 }
+LRRT_OPS_HD constexpr uint32_t attention_shared_bytes(uint32_t dim, uint32_t row_bytes,
+                                                      uint32_t heads) {
+  return attention_warps(row_bytes) *
+             (attention_stages(heads) * attention_tile_bytes(row_bytes) +
+              4u * attention_state_floats(dim, heads)) +
+         1024u;
+}
+static_assert(attention_shared_bytes(128, 256, 8) <= 232448u &&
+                  attention_shared_bytes(128, 256, 16) <= 232448u &&
+                  attention_shared_bytes(64, 256, 16) <= 232448u &&
+                  attention_shared_bytes(256, 512, 8) <= 232448u,
+              "a block's shared memory");
+// Tiles that a block takes at least, so that a short row is not split into
+// more partial states than its tiles are worth.
+constexpr uint32_t kAttentionMinimumTiles = 8;
+// Where no row has more tiles than this, blocks take whole rows: there are
+// states to join in shared memory only.
+constexpr uint32_t kAttentionWholeTiles = 32;
+// What a row costs a warp besides its tiles (its queries, and its end), in
+// tiles.
+constexpr uint32_t kAttentionRowCost = 1;
 
 struct PagedAttentionArgs {
   Rows q, out;
@@ -120,6 +131,8 @@ struct PagedAttentionArgs {
   float *states;       // [2 * grid][attention_state_floats]
   uint32_t *arrivals;  // [table.rows * rows_per_sequence], zero between launches
   uint32_t heads, group, head_dim, window;
+  uint32_t capacity; // tokens that the table holds: columns * page size
+  uint32_t paired_queries; // 16-bit q rows are multiples of 4 bytes
   uint32_t head_blocks, rows_per_sequence; // blocks of query heads per kv head; kv_heads * them
   float scale, softcap;
 };

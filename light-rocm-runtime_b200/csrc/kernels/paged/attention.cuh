@@ -5,10 +5,10 @@
 // l = l1 2^(m1 - m) + l2 2^(m2 - m), and the weighted values likewise.
 //
 // Bound by reading the cache once. What the layout does about that:
-//  - Every warp streams its own tiles (16 KB of keys and values) through three
-//    shared-memory stages filled by cp.async, so a block's four warps keep
-//    about 128 KB in flight without a barrier between them. Rows are gathered
-//    through the page table, whose entries are read one tile ahead.
+//  - Every warp streams its own tiles (8 or 16 KB of keys and values) through
+//    shared-memory stages filled by cp.async, so a block keeps about 128 KB in
+//    flight without a barrier between its warps. Rows are gathered through the
+//    page table, whose entries are read one tile ahead.
 //  - The query heads of one key-value head share each row that is read: scores
 //    are computed transposed, S^T = K Q^T, with 16 keys as the rows of the
 //    matrix product and 8 query heads as its columns, and so are the outputs,
@@ -18,10 +18,12 @@
 //    keep more than 16 bits; 32-bit operands into two TF32 parts (three
 //    products).
 //  - The tiles of all sequences and heads form one sequence that is cut into
-//    equal parts for the blocks, whatever the lengths are. A block's first and
-//    last row may be shared with its neighbours: it leaves its state in the
-//    workspace, and the last block to arrive joins the states in the blocks'
-//    order, so results do not depend on timing.
+//    equal parts for the blocks, and each part into equal parts for the warps,
+//    whatever the lengths are. A row that lies within a warp's part is finished
+//    by that warp; the pieces of others are joined in shared memory, and where
+//    a row lies in several blocks through the workspace by the last of them to
+//    arrive. Pieces are joined in their order, so that results do not depend on
+//    timing.
 #ifndef LRRT_PAGED_ATTENTION_CUH_
 #define LRRT_PAGED_ATTENTION_CUH_
 
@@ -34,7 +36,7 @@ __device__ __forceinline__ uint32_t shared_address(const void *pointer) {
 }
 
 // 16 bytes from global to shared memory; zeros where `valid` is false.
-__device__ __forceinline__ void copy_16(uint32_t to, const void *from, bool valid) {
+__device__ __forceinline__ void copy_16(uint32_t to, uint64_t from, bool valid) {
   const uint32_t bytes = valid ? 16u : 0u;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes)
                : "memory");
@@ -92,11 +94,20 @@ __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = high + low to about 22 bits, both TF32: high is x rounded to nearest
-// (half away from zero) to 11 bits, low the exact rest, rounded likewise.
+// c = a b for TF32.
+__device__ __forceinline__ void multiply_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, "
+               "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// x = high + low to about 21 bits, both TF32: high is x rounded to nearest
+// (half away from zero) to 11 bits, low the first 11 bits of the exact rest.
 __device__ __forceinline__ void split_tf32(uint32_t bits, uint32_t &high, uint32_t &low) {
   high = (bits + 0x1000u) & 0xffffe000u;
-  low = (__float_as_uint(__uint_as_float(bits) - __uint_as_float(high)) + 0x1000u) & 0xffffe000u;
+  low = __float_as_uint(__uint_as_float(bits) - __uint_as_float(high)) & 0xffffe000u;
 }
 
 // Two floats as a pair of 16-bit numbers, and what the rounding left over as
@@ -114,52 +125,23 @@ __device__ __forceinline__ void split_16(float x, float y, uint32_t &high, uint3
   low = uint32_t{a} | uint32_t{b} << 16;
 }
 
-// Which keys of a sequence a step sees, and in how many tiles.
+// The keys of a sequence that a step sees.
 struct Span {
   uint32_t begin, end;
 };
 
 __device__ __forceinline__ Span span_of(const PagedAttentionArgs &args, uint32_t sequence) {
-  const int64_t capacity = int64_t{args.table.columns} * args.cache.page.divisor;
-  int64_t end = args.lengths[sequence];
-  end = end < 0 ? 0 : end > capacity ? capacity : end;
-  const int64_t begin = args.window != 0 && end > args.window ? end - args.window : 0;
-  return {static_cast<uint32_t>(begin), static_cast<uint32_t>(end)};
+  const int32_t length = args.lengths[sequence];
+  const uint32_t end = length < 0 ? 0u : min(static_cast<uint32_t>(length), args.capacity);
+  return {args.window != 0 && end > args.window ? end - args.window : 0u, end};
 }
 
-// A place in the sequence of tiles: rows (sequence, kv head, block of query
-// heads) in order, each with the tiles of its sequence.
+// A tile and its row: a sequence, and a kv head with a block of its query heads.
 struct TileCursor {
   uint32_t sequence, row, tile; // row within the sequence; tile within the row
   uint32_t tiles;               // of the row
   Span span;
 };
-
-template <uint32_t KeysPerTile>
-__device__ __forceinline__ void enter_sequence(const PagedAttentionArgs &args, TileCursor &at) {
-  while (true) { // past empty sequences; the caller knows that tiles are left
-    at.span = span_of(args, at.sequence);
-    at.tiles = (at.span.end - at.span.begin + KeysPerTile - 1u) / KeysPerTile;
-    if (at.tiles != 0 || at.sequence + 1u >= args.table.rows) {
-      return;
-    }
-    ++at.sequence;
-  }
-}
-
-template <uint32_t KeysPerTile>
-__device__ __forceinline__ void advance(const PagedAttentionArgs &args, TileCursor &at,
-                                        uint32_t tiles) {
-  at.tile += tiles;
-  while (at.tile >= at.tiles) {
-    at.tile -= at.tiles;
-    if (++at.row == args.rows_per_sequence) {
-      at.row = 0;
-      ++at.sequence;
-      enter_sequence<KeysPerTile>(args, at);
-    }
-  }
-}
 
 template <typename T, int Dim, int HeadTiles> class PagedAttention {
   static constexpr bool kWide = sizeof(T) == 4; // 32-bit elements
@@ -167,15 +149,16 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
   static constexpr uint32_t kWarps = attention_warps(kRowBytes);
   static constexpr uint32_t kKeys = attention_tile_keys(kRowBytes);
   static constexpr uint32_t kChunks = kRowBytes / 16u; // 16-byte chunks of a row
-  static constexpr uint32_t kRowsPerPass = kChunks >= 32u ? 1u : 32u / kChunks;
+  static constexpr uint32_t kRowsPerPass = 32u / kChunks;
   static constexpr uint32_t kKeyTiles = kKeys / 16u;
-  static constexpr uint32_t kKeysPerLane = kKeys > 32u ? kKeys / 32u : 1u;
   static constexpr uint32_t kHeads = 8u * HeadTiles;
   static constexpr uint32_t kSteps = kRowBytes / 32u; // k steps of Q K^T (32 bytes of a row)
-  static constexpr uint32_t kStages = kAttentionStages;
+  static constexpr uint32_t kStages = attention_stages(8u * HeadTiles);
   static constexpr uint32_t kStageBytes = attention_tile_bytes(kRowBytes);
   static constexpr uint32_t kStateFloats = attention_state_floats(Dim, kHeads);
-  static_assert(kChunks >= 8 && kChunks <= 32 && kKeys >= 16 && kKeys <= 64, "tile shape");
+  static constexpr uint32_t kStateRow = Dim + 4u;           // floats of a head in a state
+  static constexpr uint32_t kMaximaAt = kHeads * kStateRow; // then the sums
+  static_assert(kChunks >= 8 && kChunks <= 32 && kKeys >= 16 && kKeys <= 32, "tile shape");
 
   // A row's chunk c is stored at c xor (row & 7): eight rows of a chunk column
   // then lie in different banks.
@@ -183,106 +166,163 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     return row * kRowBytes + ((chunk ^ (row & 7u)) << 4u);
   }
 
+  struct Piece { // of a row that a warp leaves unfinished
+    uint32_t row_begin, row_end; // the places of the row's tiles
+    uint32_t sequence, row, present;
+  };
+  struct HeadBlock {
+    uint32_t first, count; // query heads of a row
+  };
+
   const PagedAttentionArgs &args_;
   const uint32_t lane_ = threadIdx.x & 31u, warp_ = threadIdx.x >> 5u;
-  uint32_t ring_;           // this warp's stages
-  uint64_t *seen_;          // [kStages] which keys of the stage have a page
-  float *merge_;            // shared: states of 8 heads per warp
-  float *merge_maxima_, *merge_sums_; // [warps][8]
-  uint32_t *flag_;
+  uint32_t ring_;          // this warp's stages
+  unsigned char *rings_;   // all warps'; at the end, the states of their last pieces
+  float *states_;          // shared: [kWarps] of the pieces that began before the warp's part
+  Piece *firsts_, *lasts_; // [kWarps] of either kind
+  uint32_t *starts_;       // [kThreads] places before each thread's share; where states will be
+  uint32_t *seen_;         // [kStages] which keys of this warp's stages have a page
+  uint32_t *flags_;        // [2] whether the block joins its first, its last row
 
   uint32_t query_[HeadTiles][kSteps][kWide ? 4 : 2];
   float out_[HeadTiles][Dim / 16][4];
   float maximum_[HeadTiles][2], sum_[HeadTiles][2];
 
-  struct Gather {
-    int64_t key[kKeysPerLane], value[kKeysPerLane]; // element offsets of a lane's keys
-    bool valid[kKeysPerLane];
-  };
+  __device__ __forceinline__ uint32_t tiles_of(const Span &span) const {
+    return (span.end - span.begin + kKeys - 1u) / kKeys;
+  }
 
-  // Where the keys of a tile are, one or two of them per lane.
-  __device__ __forceinline__ void locate(const TileCursor &at, Gather &gather) const {
-    const uint32_t head = at.row / args_.head_blocks;
-#pragma unroll
-    for (uint32_t i = 0; i < kKeysPerLane; ++i) {
-      const uint32_t key = at.span.begin + at.tile * kKeys + i * 32u + (lane_ & (kKeys - 1u));
-      gather.valid[i] = key < at.span.end;
-      gather.key[i] = 0;
-      gather.value[i] = 0;
-      if (gather.valid[i]) {
-        const uint32_t column = args_.cache.page.quotient(key);
-        const uint32_t row = key - column * args_.cache.page.divisor;
-        const int32_t page = args_.table.pages[at.sequence * args_.table.row_stride + column];
-        gather.valid[i] = page >= 0 && static_cast<uint32_t>(page) < args_.cache.page_count;
-        if (gather.valid[i]) {
-          gather.key[i] = page * args_.cache.key_page + row * args_.cache.key_token +
-                          head * args_.cache.key_head;
-          gather.value[i] = page * args_.cache.value_page + row * args_.cache.value_token +
-                            head * args_.cache.value_head;
-        }
+  // The next sequence with tiles; the caller knows that there is one.
+  __device__ __forceinline__ void enter_sequence(TileCursor &at) const {
+    while (true) {
+      at.span = span_of(args_, at.sequence);
+      at.tiles = tiles_of(at.span);
+      if (at.tiles != 0 || at.sequence + 1u >= args_.table.rows) {
+        return;
       }
+      ++at.sequence;
+    }
+  }
+  __device__ __forceinline__ void next_row(TileCursor &at) const {
+    at.tile = 0;
+    if (++at.row == args_.rows_per_sequence) {
+      at.row = 0;
+      ++at.sequence;
+      enter_sequence(at);
     }
   }
 
-  __device__ __forceinline__ void issue(const Gather &gather, uint32_t stage) const {
-    const uint32_t keys = ring_ + stage * kStageBytes;
-    const uint32_t values = keys + kStageBytes / 2u;
-    const uint32_t chunk = lane_ % kChunks;
-    const bool inside = chunk * (16u / sizeof(T)) < args_.head_dim;
-    const T *key_base = static_cast<const T *>(args_.cache.keys) + chunk * (16u / sizeof(T));
-    const T *value_base = static_cast<const T *>(args_.cache.values) + chunk * (16u / sizeof(T));
-    uint64_t seen = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kKeysPerLane; ++i) {
-      seen |= uint64_t{__ballot_sync(kAllLanes, gather.valid[i])} << (32u * i);
+  __device__ __forceinline__ HeadBlock heads_of(uint32_t row) const {
+    const uint32_t kv_head = row / args_.head_blocks;
+    const uint32_t at = (row - kv_head * args_.head_blocks) * kHeads;
+    return {kv_head * args_.group + at, min(kHeads, args_.group - at)};
+  }
+
+  // Where a tile's keys are, one per lane (twice over with 16 of them).
+  struct Gather {
+    int32_t page; // -1: none
+    uint32_t row, head;
+  };
+  __device__ __forceinline__ Gather locate(const TileCursor &at) const {
+    Gather gather{-1, 0, at.row / args_.head_blocks};
+    const uint32_t key = at.span.begin + at.tile * kKeys + (lane_ & (kKeys - 1u));
+    if (key < at.span.end) {
+      const uint32_t column = args_.cache.page.quotient(key);
+      gather.row = key - column * args_.cache.page.divisor;
+      gather.page = args_.table.pages[at.sequence * args_.table.row_stride + column];
     }
+    return gather;
+  }
+
+  // Every lane works out the addresses of its key and value; a pass then copies
+  // kRowsPerPass rows of each, their addresses taken from those lanes.
+  __device__ __forceinline__ void issue(const Gather &gather, uint32_t stage) const {
+    const bool present = static_cast<uint32_t>(gather.page) < args_.cache.page_count;
+    const uint32_t seen = __ballot_sync(kAllLanes, present);
     if (lane_ == 0) {
       seen_[stage] = seen;
     }
+    const int64_t page = present ? gather.page : 0; // nothing is read there, zeros are written
+    const T *key = static_cast<const T *>(args_.cache.keys) + page * args_.cache.key_page +
+                   gather.row * args_.cache.key_token + gather.head * args_.cache.key_head;
+    const T *value = static_cast<const T *>(args_.cache.values) + page * args_.cache.value_page +
+                     gather.row * args_.cache.value_token + gather.head * args_.cache.value_head;
+    const uint32_t chunk = lane_ % kChunks;
+    const bool inside = chunk * (16u / sizeof(T)) < args_.head_dim;
+    const uint32_t offset = inside ? chunk * 16u : 0u;
+    const uint32_t wanted = inside ? seen : 0u;
+    const uint32_t keys = ring_ + stage * kStageBytes;
 #pragma unroll
     for (uint32_t pass = 0; pass < kKeys / kRowsPerPass; ++pass) {
       const uint32_t row = pass * kRowsPerPass + lane_ / kChunks;
-      const uint32_t part = pass * kRowsPerPass / 32u; // which of a lane's keys
-      const int64_t key = __shfl_sync(kAllLanes, gather.key[part], row & 31u);
-      const int64_t value = __shfl_sync(kAllLanes, gather.value[part], row & 31u);
-      const bool valid = inside && (seen >> row & 1u) != 0;
-      const uint32_t at = swizzled(row, chunk);
-      copy_16(keys + at, valid ? key_base + key : args_.cache.keys, valid);
-      copy_16(values + at, valid ? value_base + value : args_.cache.values, valid);
+      const uint64_t key_row =
+          __shfl_sync(kAllLanes, reinterpret_cast<uint64_t>(key), row) + offset;
+      const uint64_t value_row =
+          __shfl_sync(kAllLanes, reinterpret_cast<uint64_t>(value), row) + offset;
+      const bool valid = (wanted >> row & 1u) != 0;
+      const uint32_t at = keys + swizzled(row, chunk);
+      copy_16(at, key_row, valid);
+      copy_16(at + kStageBytes / 2u, value_row, valid);
+    }
+  }
+
+  // The query heads of a row, as the products' second operand: of 16-bit
+  // elements pairs, which may lie at odd places (`Paired` false).
+  template <bool Paired>
+  __device__ __forceinline__ void load_queries(uint32_t sequence, uint32_t first_head,
+                                               uint32_t heads) {
+#pragma unroll
+    for (int n = 0; n < HeadTiles; ++n) {
+      const uint32_t head = n * 8u + lane_ / 4u;
+      const T *q = static_cast<const T *>(args_.q.data) + sequence * args_.q.row_stride +
+                   (first_head + min(head, heads - 1u)) * args_.q.head_stride;
+      const uint32_t limit = head < heads ? args_.head_dim : 0u;
+#pragma unroll
+      for (uint32_t k = 0; k < kSteps; ++k) {
+#pragma unroll
+        for (uint32_t half = 0; half < 2u; ++half) {
+          if constexpr (kWide) {
+            const uint32_t d = k * 8u + half * 4u + (lane_ & 3u);
+            query_[n][k][half] = d < limit ? __float_as_uint(q[d]) : 0u;
+          } else {
+            const uint32_t d = k * 16u + half * 8u + (lane_ & 3u) * 2u;
+            if constexpr (Paired) {
+              query_[n][k][half] = d < limit ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
+            } else {
+              uint16_t low = 0, high = 0;
+              if (d < limit) {
+                memcpy(&low, q + d, 2);
+                memcpy(&high, q + d + 1u, 2);
+              }
+              query_[n][k][half] = uint32_t{low} | uint32_t{high} << 16;
+            }
+          }
+        }
+      }
+    }
+    if constexpr (kWide) {
+#pragma unroll
+      for (int n = 0; n < HeadTiles; ++n) {
+#pragma unroll
+        for (uint32_t k = 0; k < kSteps; ++k) {
+#pragma unroll
+          for (uint32_t half = 0; half < 2u; ++half) {
+            split_tf32(query_[n][k][half], query_[n][k][half], query_[n][k][2u + half]);
+          }
+        }
+      }
     }
   }
 
   __device__ __forceinline__ void begin_row(uint32_t sequence, uint32_t first_head,
                                             uint32_t heads) {
+    if (kWide || args_.paired_queries != 0) {
+      load_queries<true>(sequence, first_head, heads);
+    } else {
+      load_queries<false>(sequence, first_head, heads);
+    }
 #pragma unroll
     for (int n = 0; n < HeadTiles; ++n) {
-      const uint32_t head = n * 8u + lane_ / 4u;
-      const T *q = static_cast<const T *>(args_.q.data) + sequence * args_.q.row_stride +
-                   (first_head + head) * args_.q.head_stride;
-#pragma unroll
-      for (uint32_t k = 0; k < kSteps; ++k) {
-        if constexpr (kWide) {
-#pragma unroll
-          for (uint32_t half = 0; half < 2u; ++half) {
-            const uint32_t d = k * 8u + half * 4u + (lane_ & 3u);
-            const float x = head < heads && d < args_.head_dim ? q[d] : 0.0f;
-            split_tf32(__float_as_uint(x), query_[n][k][half], query_[n][k][2u + half]);
-          }
-        } else {
-#pragma unroll
-          for (uint32_t half = 0; half < 2u; ++half) {
-            const uint32_t d = k * 16u + half * 8u + (lane_ & 3u) * 2u;
-            uint32_t pair = 0;
-            if (head < heads && d < args_.head_dim) {
-              uint16_t low, high;
-              memcpy(&low, q + d, 2);
-              memcpy(&high, q + d + 1u, 2);
-              pair = uint32_t{low} | uint32_t{high} << 16;
-            }
-            query_[n][k][half] = pair;
-          }
-        }
-      }
 #pragma unroll
       for (int m = 0; m < Dim / 16; ++m) {
 #pragma unroll
@@ -327,8 +367,8 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
           // rounded 32 bits.
 #pragma unroll
           for (int n = 0; n < HeadTiles; ++n) {
-            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            multiply(part, low, query_[n][k][0], query_[n][k][1], T());
+            float part[4];
+            multiply_first(part, low, query_[n][k][0], query_[n][k][1]);
             multiply(part, high, query_[n][k][2], query_[n][k][3], T());
             multiply(part, high, query_[n][k][0], query_[n][k][1], T());
 #pragma unroll
@@ -344,7 +384,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
         }
       }
     }
-    const uint64_t seen = seen_[stage];
+    const uint32_t seen = seen_[stage];
     const float to_base_2 = args_.softcap > 0.0f ? args_.softcap * kLog2E : args_.scale * kLog2E;
     const float to_cap = args_.softcap > 0.0f ? args_.scale / args_.softcap : 0.0f;
 #pragma unroll
@@ -365,8 +405,10 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
           const uint32_t key = m * 16u + (i / 2) * 8u + lane_ / 4u;
           float s = score[n][m][i];
           s = args_.softcap > 0.0f ? tanhf(s * to_cap) * to_base_2 : s * to_base_2;
-          const int32_t distance = static_cast<int32_t>(end - 1u - first_key - key);
-          s -= slope[i % 2] * static_cast<float>(distance);
+          if (args_.slopes != nullptr) {
+            const int32_t distance = static_cast<int32_t>(end - 1u - first_key - key);
+            s -= slope[i % 2] * static_cast<float>(distance);
+          }
           s = (seen >> key & 1u) != 0 ? s : -INFINITY;
           score[n][m][i] = s;
           top[i % 2] = fmaxf(top[i % 2], s);
@@ -440,8 +482,8 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
             }
 #pragma unroll
             for (int n = 0; n < HeadTiles; ++n) {
-              float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-              multiply(part, low, weight[n][0], weight[n][1], T());
+              float part[4];
+              multiply_first(part, low, weight[n][0], weight[n][1]);
               multiply(part, high, weight[n][2], weight[n][3], T());
               multiply(part, high, weight[n][0], weight[n][1], T());
 #pragma unroll
@@ -478,17 +520,8 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     }
   }
 
-  __device__ __forceinline__ void store(uint32_t sequence, uint32_t head, uint32_t d,
-                                        float x) const {
-    T *out = static_cast<T *>(args_.out.data) + sequence * args_.out.row_stride +
-             head * args_.out.head_stride;
-    out[d] = from_float<T>(x);
-  }
-
-  // The warps' states of a row joined, eight heads at a time: the result
-  // where the block has the whole row (`state` null), else a partial state.
-  __device__ __forceinline__ void end_row(uint32_t sequence, uint32_t first_head, uint32_t heads,
-                                          float *state) {
+  // The sums over a warp's lanes; afterwards every lane has those of its heads.
+  __device__ __forceinline__ void sum_lanes() {
 #pragma unroll
     for (int n = 0; n < HeadTiles; ++n) {
 #pragma unroll
@@ -497,115 +530,355 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
         for (uint32_t offset = 4; offset < 32u; offset <<= 1u) {
           sum_[n][i] += __shfl_xor_sync(kAllLanes, sum_[n][i], offset);
         }
-        if (lane_ < 4u) {
-          merge_maxima_[warp_ * 8u + lane_ * 2u + i] = maximum_[n][i];
-          merge_sums_[warp_ * 8u + lane_ * 2u + i] = sum_[n][i];
-        }
       }
-#pragma unroll
-      for (int d = 0; d < Dim / 16; ++d) {
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-          const uint32_t head = (lane_ & 3u) * 2u + (i & 1u);
-          const uint32_t column = d * 16u + (i >> 1u) * 8u + lane_ / 4u;
-          merge_[(warp_ * 8u + head) * Dim + column] = out_[n][d][i];
-        }
-      }
-      __syncthreads();
-      for (uint32_t at = threadIdx.x; at < 8u * Dim; at += kThreads) {
-        const uint32_t head = at / Dim, column = at % Dim;
-        float top = -INFINITY;
-#pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) {
-          top = fmaxf(top, merge_maxima_[w * 8u + head]);
-        }
-        float sum = 0.0f, x = 0.0f;
-        const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (uint32_t w = 0; w < kWarps; ++w) {
-          const float factor = exp2_fast(merge_maxima_[w * 8u + head] - base);
-          sum += merge_sums_[w * 8u + head] * factor;
-          x += merge_[(w * 8u + head) * Dim + column] * factor;
-        }
-        const uint32_t in_row = n * 8u + head;
-        if (state != nullptr) {
-          state[in_row * Dim + column] = x;
-          if (column == 0) {
-            state[kHeads * Dim + in_row] = top;
-            state[kHeads * (Dim + 1u) + in_row] = sum;
-          }
-        } else if (in_row < heads) {
-          finish(sequence, first_head + in_row, column, x, top, sum);
-        }
-      }
-      __syncthreads();
     }
   }
 
-  __device__ __forceinline__ void finish(uint32_t sequence, uint32_t head, uint32_t column, float x,
-                                         float top, float sum) const {
-    const bool empty = top == -INFINITY;
-    if (column < args_.head_dim) {
-      store(sequence, head, column, empty ? 0.0f : x / sum);
-    }
-    if (column == 0 && args_.lse != nullptr) {
+  __device__ __forceinline__ void write_lse(uint32_t sequence, uint32_t head, float top,
+                                            float sum) const {
+    if (args_.lse != nullptr) {
       args_.lse[uint64_t{sequence} * args_.heads + head] =
-          empty ? -INFINITY : (top + log2f(sum)) * kLn2;
+          top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
     }
   }
 
-  // The states that blocks first .. last left of a row, joined by the last of
-  // them to get here. Block b left it as its last row where the row began in
-  // it, else as its first.
-  __device__ __forceinline__ void join(uint32_t sequence, uint32_t row, uint32_t first_head,
-                                       uint32_t heads, uint32_t first, uint32_t last,
-                                       uint64_t row_begin, uint64_t per_block) const {
-    __threadfence();
-    __syncthreads();
-    uint32_t *arrivals = args_.arrivals + uint64_t{sequence} * args_.rows_per_sequence + row;
-    if (threadIdx.x == 0) {
-      const bool is_last = atomicAdd(arrivals, 1u) == last - first;
-      *flag_ = is_last ? 1u : 0u;
-      if (is_last) {
-        *arrivals = 0;
+  // A row that this warp has all of.
+  __device__ __forceinline__ void finish_row(uint32_t sequence, uint32_t first_head,
+                                             uint32_t heads) const {
+#pragma unroll
+    for (int n = 0; n < HeadTiles; ++n) {
+#pragma unroll
+      for (uint32_t i = 0; i < 2u; ++i) {
+        const uint32_t head = n * 8u + (lane_ & 3u) * 2u + i;
+        if (head >= heads) {
+          continue;
+        }
+        const float top = maximum_[n][i];
+        const float inverse = top == -INFINITY ? 0.0f : 1.0f / sum_[n][i];
+        T *out = static_cast<T *>(args_.out.data) + sequence * args_.out.row_stride +
+                 (first_head + head) * args_.out.head_stride;
+#pragma unroll
+        for (uint32_t d = 0; d < Dim / 16u; ++d) {
+#pragma unroll
+          for (uint32_t half = 0; half < 2u; ++half) {
+            const uint32_t column = d * 16u + half * 8u + lane_ / 4u;
+            if (column < args_.head_dim) {
+              out[column] = from_float<T>(out_[n][d][2u * half + i] * inverse);
+            }
+          }
+        }
+        if (lane_ < 4u) {
+          write_lse(sequence, first_head + head, top, sum_[n][i]);
+        }
       }
     }
-    __syncthreads();
-    if (*flag_ == 0) {
-      __syncthreads(); // the flag may be written again
-      return;
+  }
+
+  __device__ __forceinline__ void save_state(float *state) const {
+#pragma unroll
+    for (int n = 0; n < HeadTiles; ++n) {
+#pragma unroll
+      for (uint32_t i = 0; i < 4u; ++i) {
+        const uint32_t head = n * 8u + (lane_ & 3u) * 2u + (i & 1u);
+#pragma unroll
+        for (uint32_t d = 0; d < Dim / 16u; ++d) {
+          state[head * kStateRow + d * 16u + (i >> 1u) * 8u + lane_ / 4u] = out_[n][d][i];
+        }
+        if (lane_ < 4u && i < 2u) {
+          state[kMaximaAt + head] = maximum_[n][i];
+          state[kMaximaAt + kHeads + head] = sum_[n][i];
+        }
+      }
     }
-    __threadfence();
-    const uint32_t count = last - first + 1u;
-    auto state_of = [&](uint32_t i) {
-      const uint32_t block = first + i;
-      const uint32_t slot = row_begin >= block * per_block ? 1u : 0u;
-      return args_.states + (2u * uint64_t{block} + slot) * kStateFloats;
+  }
+
+  // Four columns of a head, joined from several states: unscaled, with their
+  // maximum and sum.
+  struct Joined {
+    float4 x;
+    float top, sum;
+
+    __device__ __forceinline__ void add_state(const float *state, uint32_t head,
+                                              uint32_t column) {
+      const float other = state[kMaximaAt + head];
+      const float other_sum = state[kMaximaAt + kHeads + head];
+      const float4 y = *reinterpret_cast<const float4 *>(state + head * kStateRow + column);
+      const float now = fmaxf(top, other);
+      const float base = now == -INFINITY ? 0.0f : now;
+      const float mine = exp2_fast(top - base), theirs = exp2_fast(other - base);
+      x = {x.x * mine + y.x * theirs, x.y * mine + y.y * theirs, x.z * mine + y.z * theirs,
+           x.w * mine + y.w * theirs};
+      sum = sum * mine + other_sum * theirs;
+      top = now;
+    }
+  };
+
+  __device__ __forceinline__ void finish(uint32_t sequence, uint32_t head, uint32_t column,
+                                         const Joined &joined) const {
+    const float inverse = joined.top == -INFINITY ? 0.0f : 1.0f / joined.sum;
+    T *out = static_cast<T *>(args_.out.data) + sequence * args_.out.row_stride +
+             head * args_.out.head_stride;
+    const float x[4] = {joined.x.x, joined.x.y, joined.x.z, joined.x.w};
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; ++i) {
+      if (column + i < args_.head_dim) {
+        out[column + i] = from_float<T>(x[i] * inverse);
+      }
+    }
+    if (column == 0) {
+      write_lse(sequence, head, joined.top, joined.sum);
+    }
+  }
+
+  // The pieces of one row that the block's warps left, from `warp` on: its
+  // last one, or its first for a row from before the block. A row that other
+  // blocks have a part of goes to `part`. By `threads` threads, this one the
+  // `thread`th.
+  __device__ __forceinline__ void join_pieces(const Piece &piece, uint32_t warp, bool from_last,
+                                              float *part, uint32_t thread, uint32_t threads) {
+    uint32_t count = 1;
+    while (warp + count < kWarps && firsts_[warp + count].present != 0 &&
+           firsts_[warp + count].row_begin == piece.row_begin) {
+      ++count;
+    }
+    const float *first_state =
+        from_last ? reinterpret_cast<const float *>(rings_ + warp * kStages * kStageBytes)
+                  : states_ + warp * kStateFloats;
+    const HeadBlock heads = heads_of(piece.row);
+#pragma unroll 1
+    for (uint32_t at = thread * 4u; at < heads.count * Dim; at += threads * 4u) {
+      const uint32_t head = at / Dim, column = at % Dim;
+      Joined joined{{0.0f, 0.0f, 0.0f, 0.0f}, -INFINITY, 0.0f};
+      const float *state = first_state;
+#pragma unroll 2
+      for (uint32_t i = 0; i < count; ++i) {
+        joined.add_state(state, head, column);
+        state = states_ + (warp + i + 1u) * kStateFloats;
+      }
+      if (part == nullptr) {
+        finish(piece.sequence, heads.first + head, column, joined);
+      } else {
+        *reinterpret_cast<float4 *>(part + head * kStateRow + column) = joined.x;
+        if (column == 0) {
+          part[kMaximaAt + head] = joined.top;
+          part[kMaximaAt + kHeads + head] = joined.sum;
+        }
+      }
+    }
+  }
+
+  // The state that block `block` leaves of a row of several: its last where
+  // the row begins in it, else its first.
+  __device__ __forceinline__ float *part_of(uint32_t block, bool begins) const {
+    return args_.states + (2u * size_t{block} + (begins ? 1u : 0u)) * kStateFloats;
+  }
+
+  __device__ __forceinline__ uint32_t parts_of(const Piece &piece, uint32_t per_block) const {
+    return (piece.row_end - 1u) / per_block - piece.row_begin / per_block + 1u;
+  }
+
+  // The parts that the blocks left of a row, all of them there by now: brought
+  // into the rings, which are free, as many at a time as these hold.
+  __device__ __forceinline__ void join_parts(const Piece &piece, uint32_t per_block) const {
+    const uint32_t first = piece.row_begin / per_block, count = parts_of(piece, per_block);
+    const HeadBlock heads = heads_of(piece.row);
+    constexpr uint32_t kRound = kWarps * kStages * kStageBytes / (4u * kStateFloats);
+    constexpr uint32_t kItems = kHeads * Dim / 4u;
+    constexpr uint32_t kEach = (kItems + kThreads - 1u) / kThreads;
+    const float *staged = reinterpret_cast<const float *>(rings_);
+    Joined joined[kEach];
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+      joined[j] = {{0.0f, 0.0f, 0.0f, 0.0f}, -INFINITY, 0.0f};
+    }
+#pragma unroll 1
+    for (uint32_t begin = 0; begin < count; begin += kRound) {
+      const uint32_t now = min(kRound, count - begin);
+#pragma unroll 1
+      for (uint32_t i = warp_; i < now; i += kWarps) {
+        const uint64_t from =
+            reinterpret_cast<uint64_t>(part_of(first + begin + i, begin + i == 0));
+        const uint32_t to = shared_address(staged + i * kStateFloats);
+#pragma unroll 4
+        for (uint32_t at = lane_; at < kStateFloats / 4u; at += 32u) {
+          copy_16(to + at * 16u, from + at * 16u, true);
+        }
+      }
+      commit_copies();
+      wait_copies<0>();
+      __syncthreads();
+#pragma unroll
+      for (uint32_t j = 0; j < kEach; ++j) {
+        const uint32_t at = (threadIdx.x + j * kThreads) * 4u;
+        if (at < heads.count * Dim) {
+#pragma unroll 4
+          for (uint32_t i = 0; i < now; ++i) {
+            joined[j].add_state(staged + i * kStateFloats, at / Dim, at % Dim);
+          }
+        }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+      const uint32_t at = (threadIdx.x + j * kThreads) * 4u;
+      if (at < heads.count * Dim) {
+        finish(piece.sequence, heads.first + at / Dim, at % Dim, joined[j]);
+      }
+    }
+  }
+
+  // Where warp w's tiles begin: equal parts, empty ones at the end alone.
+  static __device__ __forceinline__ uint32_t warp_part(uint32_t begin, uint32_t count,
+                                                       uint32_t w) {
+    return begin + count / kWarps * w + min(w, count % kWarps);
+  }
+
+  // Places: the tiles of all rows one after another, each row's followed by
+  // kAttentionRowCost places that stand for the work a row takes besides its
+  // tiles. Blocks and warps take equal numbers of places.
+  __device__ __forceinline__ uint32_t places_of(uint32_t sequence) const {
+    const uint32_t tiles = tiles_of(span_of(args_, sequence));
+    return tiles == 0 ? 0u : (tiles + kAttentionRowCost) * args_.rows_per_sequence;
+  }
+
+  // The sequence of a place and the places before it, from the sums before
+  // each thread's share (in shared memory, at the start). For whole warps.
+  struct Start {
+    uint32_t sequence, before;
+  };
+  __device__ __forceinline__ Start find(uint32_t place, uint32_t share) const {
+    constexpr uint32_t kEach = kThreads / 32u;
+    // The last thread with no more than `place` before it: a group of threads
+    // per lane, then the group's threads.
+    const uint32_t groups = __ballot_sync(kAllLanes, starts_[lane_ * kEach] <= place);
+    const uint32_t group = 31u - __clz(groups);
+    const uint32_t threads =
+        __ballot_sync(kAllLanes, lane_ < kEach && starts_[group * kEach + lane_ % kEach] <= place);
+    const uint32_t thread = group * kEach + 31u - __clz(threads);
+    Start start{thread * share, starts_[thread]};
+#pragma unroll 1
+    while (true) {
+      const uint32_t places = places_of(start.sequence);
+      if (place - start.before < places) {
+        return start;
+      }
+      start.before += places;
+      ++start.sequence;
+    }
+  }
+
+  // The place where the next row begins, or this one where it is one.
+  __device__ __forceinline__ uint32_t row_boundary(uint32_t place, uint32_t total,
+                                                   uint32_t share) const {
+    if (place >= total) {
+      return total;
+    }
+    const Start start = find(place, share);
+    const uint32_t row = tiles_of(span_of(args_, start.sequence)) + kAttentionRowCost;
+    return start.before + (place - start.before + row - 1u) / row * row;
+  }
+
+  // A warp's tiles, between the places begin and end, each loaded kStages - 1
+  // steps ahead, and their page numbers two more.
+  __device__ __forceinline__ void run_warp(uint32_t begin, uint32_t end, const Start &start) {
+    TileCursor at; // the tile to compute
+    at.sequence = start.sequence;
+    at.span = span_of(args_, at.sequence);
+    at.tiles = tiles_of(at.span);
+    at.row = (begin - start.before) / (at.tiles + kAttentionRowCost);
+    uint32_t row_begin = start.before + at.row * (at.tiles + kAttentionRowCost);
+    at.tile = begin - row_begin;
+    uint32_t tile = begin; // the place of the tile to compute
+    if (at.tile >= at.tiles) { // past the row's last
+      tile = row_begin = row_begin + at.tiles + kAttentionRowCost;
+      if (tile >= end) {
+        return;
+      }
+      next_row(at);
+    }
+    uint32_t row_end = row_begin + at.tiles;
+    TileCursor load_at = at;
+    Gather gather = locate(load_at), gather_after = gather;
+    // The tile to load and the one to look up, `ahead` the place of the latter;
+    // past the end there are none.
+    uint32_t ahead = tile;
+    bool load = true, load_after = true;
+    auto look_up = [&]() {
+      if (load_after) {
+        ++ahead;
+        if (++load_at.tile == load_at.tiles) {
+          ahead += kAttentionRowCost;
+          if (ahead < end) {
+            next_row(load_at);
+          }
+        }
+        load_after = ahead < end;
+        if (load_after) {
+          gather_after = locate(load_at);
+        }
+      }
     };
-    // Weights [head][state] in the merge area, as far as it reaches.
-    float *weights = merge_;
-    for (uint32_t at = threadIdx.x; at < kHeads * count; at += kThreads) {
-      weights[at] = __ldcg(state_of(at % count) + kHeads * Dim + at / count);
-    }
-    __syncthreads();
-    for (uint32_t at = threadIdx.x; at < heads * Dim; at += kThreads) {
-      const uint32_t head = at / Dim;
-      float top = -INFINITY;
-      for (uint32_t i = 0; i < count; ++i) {
-        top = fmaxf(top, weights[head * count + i]);
+    look_up();
+    uint32_t load_stage = 0, stage = 0;
+    HeadBlock heads = heads_of(at.row);
+    bool entered = false;
+#pragma unroll 1
+    for (uint32_t step = 0; tile < end; ++step) {
+      if (!entered) {
+        begin_row(at.sequence, heads.first, heads.count);
+        entered = true;
       }
-      const float base = top == -INFINITY ? 0.0f : top;
-      float x = 0.0f, sum = 0.0f;
-#pragma unroll 8
-      for (uint32_t i = 0; i < count; ++i) {
-        const float *state = state_of(i);
-        const float factor = exp2_fast(weights[head * count + i] - base);
-        x += __ldcg(state + at) * factor;
-        sum += __ldcg(state + kHeads * (Dim + 1u) + head) * factor;
+      if (load) {
+        issue(gather, load_stage);
+        gather = gather_after;
+        load = load_after;
+        look_up();
       }
-      finish(sequence, first_head + head, at % Dim, x, top, sum);
+      commit_copies();
+      load_stage = load_stage + 1u == kStages ? 0u : load_stage + 1u;
+      if (step + 1u < kStages) {
+        continue; // not all stages are under way yet
+      }
+      wait_copies<kStages - 1>();
+      __syncwarp();
+      compute(stage, at.span.begin + (tile - row_begin) * kKeys, at.span.end, heads.first,
+              heads.count);
+      __syncwarp(); // the stage is filled again by the next issue
+      stage = stage + 1u == kStages ? 0u : stage + 1u;
+      ++tile;
+      if (tile != row_end && tile != end) {
+        continue;
+      }
+      sum_lanes();
+      if (row_begin >= begin && row_end <= end) {
+        finish_row(at.sequence, heads.first, heads.count);
+      } else {
+        // A row from before the warp's part is its first; one that goes on
+        // past it is its last, and nothing is left to load then.
+        const bool is_first = row_begin < begin;
+        if (!is_first) {
+          wait_copies<0>();
+          __syncwarp();
+        }
+        save_state(is_first ? states_ + warp_ * kStateFloats
+                            : reinterpret_cast<float *>(rings_ + warp_ * kStages * kStageBytes));
+        if (lane_ == 0) {
+          (is_first ? firsts_ : lasts_)[warp_] = {row_begin, row_end, at.sequence, at.row, 1u};
+        }
+      }
+      if (tile != row_end) {
+        break; // the row goes on past the end
+      }
+      tile = row_begin = row_end + kAttentionRowCost;
+      if (tile < end) {
+        next_row(at);
+        row_end = row_begin + at.tiles;
+        heads = heads_of(at.row);
+        entered = false;
+      }
     }
-    __syncthreads();
+    wait_copies<0>();
   }
 
 public:
@@ -613,148 +886,138 @@ public:
 
   __device__ __forceinline__ PagedAttention(const PagedAttentionArgs &args, unsigned char *shared)
       : args_(args) {
+    rings_ = shared;
     ring_ = shared_address(shared) + warp_ * kStages * kStageBytes;
     unsigned char *at = shared + kWarps * kStages * kStageBytes;
-    merge_ = reinterpret_cast<float *>(at);
-    at += 4u * attention_merge_floats(Dim, kRowBytes);
-    merge_maxima_ = reinterpret_cast<float *>(at);
-    merge_sums_ = merge_maxima_ + kWarps * 8u;
-    seen_ = reinterpret_cast<uint64_t *>(merge_sums_ + kWarps * 8u) + warp_ * kStages;
-    at += 2u * 4u * kWarps * 8u + 8u * kWarps * kStages;
-    flag_ = reinterpret_cast<uint32_t *>(at);
+    states_ = reinterpret_cast<float *>(at);
+    at += 4u * kWarps * kStateFloats;
+    firsts_ = reinterpret_cast<Piece *>(at);
+    lasts_ = firsts_ + kWarps;
+    starts_ = reinterpret_cast<uint32_t *>(states_);
+    seen_ = reinterpret_cast<uint32_t *>(lasts_ + kWarps) + warp_ * kStages;
+    flags_ = reinterpret_cast<uint32_t *>(lasts_ + kWarps) + kWarps * kStages;
+    static_assert(2u * sizeof(Piece) * kWarps + 4u * kStages * kWarps + 8u <= 1024u &&
+                      kThreads + 2u * kWarps <= kWarps * kStateFloats,
+                  "shared memory of the bookkeeping");
   }
 
   __device__ __forceinline__ void run() {
-    // Tiles before each thread's share of the sequences, and of all of them.
+    // Places before each thread's share of the sequences, and all of them.
     const uint32_t share = (args_.table.rows + kThreads - 1u) / kThreads;
     const uint32_t mine_begin = min(threadIdx.x * share, args_.table.rows);
     const uint32_t mine_end = min(mine_begin + share, args_.table.rows);
-    uint64_t mine = 0;
+    uint32_t mine = 0;
+#pragma unroll 1
     for (uint32_t s = mine_begin; s < mine_end; ++s) {
-      const Span span = span_of(args_, s);
-      mine += uint64_t{(span.end - span.begin + kKeys - 1u) / kKeys} * args_.rows_per_sequence;
+      mine += places_of(s);
     }
-    uint64_t *sums = reinterpret_cast<uint64_t *>(merge_); // [warps], then the block's start
-    uint64_t upto = mine;
+    uint32_t upto = mine, most = mine; // inclusive sums; places of the sequence with most
 #pragma unroll
     for (uint32_t offset = 1; offset < 32u; offset <<= 1u) {
-      const uint64_t other = __shfl_up_sync(kAllLanes, upto, offset);
-      upto += lane_ >= offset ? other : 0;
+      const uint32_t other = __shfl_up_sync(kAllLanes, upto, offset);
+      upto += lane_ >= offset ? other : 0u;
+      most = max(most, __shfl_xor_sync(kAllLanes, most, offset));
     }
+    uint32_t *warp_sums = starts_ + kThreads;
     if (lane_ == 31u) {
-      sums[warp_] = upto;
+      warp_sums[warp_] = upto;
+      warp_sums[kWarps + warp_] = most;
+      firsts_[warp_].present = 0;
+      lasts_[warp_].present = 0;
     }
     __syncthreads();
-    uint64_t before = upto - mine, total = 0;
+    uint32_t before = upto - mine, total = 0;
 #pragma unroll
     for (uint32_t w = 0; w < kWarps; ++w) {
-      before += w < warp_ ? sums[w] : 0;
-      total += sums[w];
+      const uint32_t sum = warp_sums[w];
+      before += w < warp_ ? sum : 0u;
+      total += sum;
+      most = max(most, warp_sums[kWarps + w]);
+    }
+    starts_[threadIdx.x] = before;
+    __syncthreads();
+    const uint32_t per_block =
+        max((total + gridDim.x - 1u) / gridDim.x, kAttentionMinimumTiles);
+    uint32_t begin = min(blockIdx.x * per_block, total);
+    uint32_t end = min(begin + per_block, total);
+    if (share == 1u &&
+        most <= (kAttentionWholeTiles + kAttentionRowCost) * args_.rows_per_sequence) {
+      begin = row_boundary(begin, total, share);
+      end = row_boundary(end, total, share);
+    }
+    const uint32_t count = end - begin;
+    const uint32_t warp_begin = warp_part(begin, count, warp_);
+    const uint32_t warp_end = warp_part(begin, count, warp_ + 1u);
+    Start start{0, 0};
+    if (warp_begin < warp_end) {
+      start = find(warp_begin, share);
+    }
+    __syncthreads(); // the starts lie where states will
+    if (warp_begin < warp_end) {
+      run_warp(warp_begin, warp_end, start);
     }
     __syncthreads();
-    uint64_t per_block = (total + gridDim.x - 1u) / gridDim.x;
-    per_block = per_block < kAttentionMinimumTiles ? kAttentionMinimumTiles : per_block;
-    const uint64_t begin = blockIdx.x * per_block;
-    const uint64_t end = begin + per_block < total ? begin + per_block : total;
-    if (begin < total && begin >= before && begin < before + mine) {
-      uint32_t s = mine_begin;
-      while (true) {
-        const Span span = span_of(args_, s);
-        const uint64_t tiles =
-            uint64_t{(span.end - span.begin + kKeys - 1u) / kKeys} * args_.rows_per_sequence;
-        if (begin < before + tiles) {
-          break;
-        }
-        before += tiles;
-        ++s;
+    // Rows from before the block (i = 0), then those that begin in warp i - 1:
+    // one or two by all threads, more of them a warp each.
+    const uint32_t present = __ballot_sync(
+        kAllLanes, lane_ <= kWarps &&
+                       (lane_ == 0 ? firsts_[0] : lasts_[lane_ - 1u]).present != 0);
+    const bool by_warp = __popc(present) > 2;
+    uint32_t go_on[2] = {kWarps + 1u, kWarps + 1u}; // those of other blocks too
+    uint32_t turn = 0;
+#pragma unroll 1
+    for (uint32_t left = present; left != 0; left &= left - 1u, ++turn) {
+      const uint32_t i = __ffs(left) - 1u;
+      const Piece &piece = i == 0 ? firsts_[0] : lasts_[i - 1u];
+      const bool begins = piece.row_begin >= begin;
+      const bool whole = begins && piece.row_end <= end;
+      if (!whole) {
+        go_on[begins ? 1 : 0] = i;
       }
-      sums[0] = s;
-      sums[1] = before;
+      if (!by_warp || turn % kWarps == warp_) {
+        join_pieces(piece, i == 0 ? 0u : i - 1u, i != 0,
+                    whole ? nullptr : part_of(blockIdx.x, begins),
+                    by_warp ? lane_ : threadIdx.x, by_warp ? 32u : kThreads);
+      }
+    }
+    // Where this block is the last to leave its part of a row, it joins them.
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x < 2u) {
+      const uint32_t i = threadIdx.x == 0 ? go_on[0] : go_on[1];
+      uint32_t last = 0;
+      if (i <= kWarps) {
+        const Piece &piece = i == 0 ? firsts_[0] : lasts_[i - 1u];
+        uint32_t *arrivals =
+            args_.arrivals + size_t{piece.sequence} * args_.rows_per_sequence + piece.row;
+        last = atomicAdd(arrivals, 1u) + 1u == parts_of(piece, per_block) ? 1u : 0u;
+        if (last != 0) {
+          *arrivals = 0;
+        }
+      }
+      flags_[threadIdx.x] = last;
+    }
+    __syncthreads();
+    __threadfence();
+#pragma unroll 1
+    for (uint32_t which = 0; which < 2u; ++which) {
+      if (flags_[which] != 0) {
+        const uint32_t i = which == 0 ? go_on[0] : go_on[1];
+        join_parts(i == 0 ? firsts_[0] : lasts_[i - 1u], per_block);
+      }
     }
     // Rows of sequences that see nothing.
+#pragma unroll 1
     for (uint32_t s = blockIdx.x; s < args_.table.rows; s += gridDim.x) {
       const Span span = span_of(args_, s);
       if (span.begin == span.end) {
-        for (uint32_t at = threadIdx.x; at < args_.heads * Dim; at += kThreads) {
-          finish(s, at / Dim, at % Dim, 0.0f, -INFINITY, 0.0f);
+        const Joined none{{0.0f, 0.0f, 0.0f, 0.0f}, -INFINITY, 0.0f};
+#pragma unroll 1
+        for (uint32_t at = threadIdx.x * 4u; at < args_.heads * Dim; at += kThreads * 4u) {
+          finish(s, at / Dim, at % Dim, none);
         }
       }
     }
-    __syncthreads();
-    if (begin >= total) {
-      return;
-    }
-    TileCursor row_at; // the row that the block is at; tile: where it begins
-    row_at.sequence = static_cast<uint32_t>(sums[0]);
-    const uint64_t before_sequence = sums[1];
-    __syncthreads();
-    enter_sequence<kKeys>(args_, row_at);
-    row_at.row = static_cast<uint32_t>((begin - before_sequence) / row_at.tiles);
-    row_at.tile = static_cast<uint32_t>((begin - before_sequence) % row_at.tiles);
-    uint64_t row_begin = begin - row_at.tile;
-
-    // This warp's tiles are begin + warp, + 4, ...: `next` is the one to load.
-    TileCursor load_at = row_at;
-    uint64_t next = begin + warp_;
-    Gather gather;
-    if (next < end) {
-      advance<kKeys>(args_, load_at, warp_);
-      locate(load_at, gather);
-    }
-    uint32_t load_stage = 0, stage = 0;
-    auto issue_next = [&]() {
-      if (next < end) {
-        issue(gather, load_stage);
-        next += kWarps;
-        if (next < end) {
-          advance<kKeys>(args_, load_at, kWarps);
-          locate(load_at, gather);
-        }
-      }
-      commit_copies();
-      load_stage = load_stage + 1u == kStages ? 0u : load_stage + 1u;
-    };
-#pragma unroll
-    for (uint32_t i = 0; i + 1u < kStages; ++i) {
-      issue_next();
-    }
-    uint64_t tile = begin + warp_;
-    while (true) {
-      const uint64_t row_end = row_begin + row_at.tiles;
-      const uint64_t stop = row_end < end ? row_end : end;
-      const uint32_t kv_head = row_at.row / args_.head_blocks;
-      const uint32_t block_head = (row_at.row - kv_head * args_.head_blocks) * kHeads;
-      const uint32_t first_head = kv_head * args_.group + block_head;
-      const uint32_t heads = min(kHeads, args_.group - block_head);
-      begin_row(row_at.sequence, first_head, heads);
-      for (; tile < stop; tile += kWarps) {
-        issue_next();
-        wait_copies<kStages - 1>();
-        __syncwarp();
-        compute(stage,
-                row_at.span.begin + static_cast<uint32_t>(tile - row_begin) * kKeys,
-                row_at.span.end, first_head, heads);
-        __syncwarp(); // the stage is filled again by the next issue
-        stage = stage + 1u == kStages ? 0u : stage + 1u;
-      }
-      const uint32_t first = static_cast<uint32_t>(row_begin / per_block);
-      const uint32_t last = static_cast<uint32_t>((row_end - 1u) / per_block);
-      if (first == last) {
-        end_row(row_at.sequence, first_head, heads, nullptr);
-      } else {
-        const uint32_t slot = row_begin >= begin ? 1u : 0u;
-        end_row(row_at.sequence, first_head, heads,
-                args_.states + (2u * uint64_t{blockIdx.x} + slot) * kStateFloats);
-        join(row_at.sequence, row_at.row, first_head, heads, first, last, row_begin, per_block);
-      }
-      if (row_end >= end) {
-        break;
-      }
-      row_begin = row_end;
-      row_at.tile = row_at.tiles;
-      advance<kKeys>(args_, row_at, 0);
-    }
-    wait_copies<0>();
   }
 };
 

@@ -300,19 +300,22 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
   args.group = group;
   args.head_dim = a.cache.head_dim;
   args.window = a.window;
+  args.paired_queries = rows_take(a.q, element, 4) ? 1u : 0u;
   args.head_blocks = static_cast<uint32_t>(ceil_div(group, heads));
   args.rows_per_sequence = a.cache.kv_heads * args.head_blocks;
   args.scale = a.scale;
   args.softcap = a.softcap;
 
   uint64_t tokens = uint64_t{a.table.columns} * a.cache.page_size;
+  args.capacity = static_cast<uint32_t>(tokens);
   if (a.window != 0) {
     tokens = std::min<uint64_t>(tokens, a.window);
   }
   const uint64_t rows = uint64_t{a.table.rows} * args.rows_per_sequence;
   const uint32_t row_bytes = dim * static_cast<uint32_t>(element);
   const uint32_t keys = attention_tile_keys(row_bytes);
-  const uint64_t tiles = rows * ceil_div(tokens, keys);
+  const uint64_t tiles = rows * (ceil_div(tokens, keys) + kAttentionRowCost);
+  require(tiles < (uint64_t{1} << 31), "the table's tokens, times the kv heads, are too many");
   const uint32_t grid = static_cast<uint32_t>(
       std::clamp<uint64_t>(ceil_div(tiles, kAttentionMinimumTiles), 1u, context.sms));
   context.reserve(size_t{8} * grid * attention_state_floats(dim, heads));
@@ -321,7 +324,8 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
   args.arrivals = static_cast<uint32_t *>(context.counters->data());
   context.launch(std::string("ops_attention_") + type_name(a.cache.type) + "_" +
                      std::to_string(dim) + "x" + std::to_string(heads),
-                 grid, 32u * attention_warps(row_bytes), attention_shared_bytes(dim, row_bytes), args);
+                 grid, 32u * attention_warps(row_bytes), attention_shared_bytes(dim, row_bytes, heads),
+                 args);
 }
 
 // Checks the pool and fills what its moves share; returns whether 16-byte
