@@ -7,6 +7,7 @@ Outputs (git-ignored, shipped with the working tree):
   lib/qwen_prefill.cubin          sm_100a prompt prefill kernels
   lib/decoder_ops.cubin + .json   per-operation decode kernels as an lrrt::bundle
   lib/liblrrt_ops.so              paged-cache operators (include/lrrt_ops.h)
+  lib/lrrt_ops_torch.so           the same on torch tensors, a Python extension
   lib/paged_ops.cubin             their sm_100a kernels
   _build/tests/stateful_graph_fixture.cubin  sm_100a scheduler fixture kernels (tests)
   _build/tests/*                  C++ host tests (tests/cpp)
@@ -53,6 +54,22 @@ def _run(command: list[str], verbose: bool) -> None:
     subprocess.run(command, check=True)
 
 
+def _torch_flags() -> list[str]:
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    return [f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            *(f"-isystem{path}" for path in
+              (*include_paths(), sysconfig.get_paths()["include"]))]
+
+
+def _torch_libraries() -> list[str]:
+    from torch.utils.cpp_extension import library_paths
+    return [*(f"-L{path}" for path in library_paths()), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+            "-ltorch_python"]
+
+
 def build(verbose: bool = False) -> dict[str, Path]:
     LIB.mkdir(exist_ok=True)
     BUILD.mkdir(exist_ok=True)
@@ -89,11 +106,20 @@ def build(verbose: bool = False) -> dict[str, Path]:
 
     # Paged-cache operators (include/lrrt_ops.h).
     ops = LIB / "liblrrt_ops.so"
-    ops_sources = sorted((csrc / "ops").glob("*.cpp"))
+    ops_sources = [csrc / "ops" / "ops.cpp"]
     if _stale(ops, ops_sources + headers + [runtime]):
         _run([CXX, *CXXFLAGS, "-shared", "-fvisibility=hidden", *map(str, ops_sources), "-o",
               str(ops), f"-L{LIB}", "-llrrt", "-Wl,-rpath,$ORIGIN"], verbose)
     outputs["ops"] = ops
+
+    # The operators on torch tensors (lrrt_b200/ops.py): a Python extension.
+    binding = LIB / "lrrt_ops_torch.so"
+    binding_source = csrc / "ops" / "torch_binding.cpp"
+    if _stale(binding, [binding_source] + headers + [ops]):
+        _run([CXX, *CXXFLAGS, *_torch_flags(), "-shared", "-fvisibility=hidden",
+              str(binding_source), "-o", str(binding), f"-L{LIB}", "-llrrt_ops", "-llrrt",
+              *_torch_libraries(), "-Wl,-rpath,$ORIGIN"], verbose)
+    outputs["ops_torch"] = binding
 
     for name in ("qwen_stateful_graph", "qwen_prefill", "decoder_ops", "paged_ops"):
         source = csrc / "kernels" / f"{name}.cu"

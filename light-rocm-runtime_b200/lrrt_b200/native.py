@@ -17,6 +17,7 @@ LIB = PACKAGE / "lib"
 RUNTIME_PATH = LIB / "liblrrt.so"
 DRIVER_PATH = LIB / "liblrrt_qwen.so"
 OPS_PATH = LIB / "liblrrt_ops.so"
+OPS_TORCH_PATH = LIB / "lrrt_ops_torch.so"
 OPS_CUBIN = LIB / "paged_ops.cubin"
 QWEN_CUBIN = LIB / "qwen_stateful_graph.cubin"
 PREFILL_CUBIN = LIB / "qwen_prefill.cubin"
