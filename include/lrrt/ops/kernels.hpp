@@ -194,8 +194,22 @@ struct MoveArgs {
 };
 
 constexpr uint32_t kBeamThreads = 256;
+constexpr uint32_t kBeamBlocksPerSm = 3;
 constexpr uint32_t kBeamMaximumCount = 64;
 constexpr uint32_t kBeamMaximumCandidates = 2048; // beams * count
+// Elements that a block reads at a time: 16 KB.
+LRRT_OPS_HD constexpr uint32_t beam_round(uint32_t element_bytes) {
+  return 16384u / element_bytes;
+}
+constexpr uint32_t kBeamPool = 2048;              // candidates it holds
+constexpr uint32_t kBeamMaximumParts = 64;        // of a row
+constexpr uint32_t kBeamNotedRounds = 24;         // of a part
+constexpr uint32_t kBeamMaximumVocab = 1u << 21;
+static_assert(kBeamMaximumVocab <= kBeamNotedRounds * beam_round(4) *
+                                       (kBeamPool / kBeamMaximumCount),
+              "the parts of the longest row hold it");
+constexpr uint32_t kBeamSharedBytes = 46080;
+static_assert(kBeamMaximumCandidates <= kBeamPool, "a group's candidates fit the pool");
 
 struct Pair {
   float x, y;
@@ -209,10 +223,11 @@ struct BeamArgs {
   float *scores_out;
   int32_t *parents_out, *tokens_out;
   uint8_t *finished_out;
-  uint32_t groups, beams, vocab, count, chunks;
+  uint32_t groups, beams, vocab, count;
+  uint32_t parts, part_elements; // of a row; elements a multiple of 8
   int32_t end_token;
-  uint64_t *chunk_keys;   // [rows][chunks][count]
-  Pair *chunk_sums;       // [rows][chunks] maximum, sum of exponentials
+  uint64_t *part_keys;    // [rows][parts][count]
+  Pair *part_sums;        // [rows][parts] maximum, sum of exponentials
   uint64_t *row_keys;     // [rows][count]
   float *row_log_sums;    // [rows]
   uint32_t *row_arrivals; // [rows], zero between launches

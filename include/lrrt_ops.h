@@ -226,8 +226,8 @@ LRRT_API lr_status_t lro_pages_copy(lro_context_t *context, const lro_pages_copy
  *   parents_out = g * beams + k, as lro_pages_fork takes them
  *   finished_out = the beam was finished, or the token is end_token
  * With count = beams, scores_out and finished_out may be scores and finished.
- * Outputs are [groups][count]; beams and count: 1 to 64, count <= vocab, and
- * beams * count <= 2048.
+ * Outputs are [groups][count]; beams and count: 1 to 64, their product at most
+ * 2048; count <= vocab <= 2^21; groups * beams <= 65535.
  */
 typedef struct lro_beam_select_t {
   const void *logits; /* [groups * beams][vocab] */

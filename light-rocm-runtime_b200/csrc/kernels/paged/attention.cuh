@@ -981,9 +981,9 @@ public:
       }
     }
     // Where this block is the last to leave its part of a row, it joins them.
-    __threadfence();
     __syncthreads();
     if (threadIdx.x < 2u) {
+      __threadfence(); // what the barrier showed this thread, to the whole GPU
       const uint32_t i = threadIdx.x == 0 ? go_on[0] : go_on[1];
       uint32_t last = 0;
       if (i <= kWarps) {
@@ -996,9 +996,9 @@ public:
         }
       }
       flags_[threadIdx.x] = last;
+      __threadfence();
     }
     __syncthreads();
-    __threadfence();
 #pragma unroll 1
     for (uint32_t which = 0; which < 2u; ++which) {
       if (flags_[which] != 0) {

@@ -1,14 +1,21 @@
 // The best continuations over the beams of a group and the vocabulary.
 //
-// One pass over the logits: a block reads a chunk of a row into registers,
-// takes the chunk's maximum m and sum of exp(x - m), and its `count` best
-// elements; the last block of a row joins the chunks (sums by
-// l1 e^(m1 - m) + l2 e^(m2 - m)), the last row of a group ranks the beams'
-// candidates by score + logit - log sum. Bound by reading the logits once.
+// One pass over the logits. A block reads a part of a row, 16 KB a round. Each
+// thread keeps a running maximum and sum of exponentials (sums of disjoint
+// elements join as l1 e^(m1 - m) + l2 e^(m2 - m)), and notes the maximum of
+// each round. The threads' maxima give a floor that at least `count` elements
+// reach and few others; those few are read once more (from the caches, and only
+// where a noted maximum reaches the floor) and ranked. The last block of a row
+// joins the parts, the last row of a group ranks the beams' candidates by
+// score + logit - log sum.
 //
-// Elements are compared as 64-bit keys, the value's order in the upper half
-// and the complement of the index in the lower, so that no two are equal and
-// the order of threads and blocks decides nothing.
+// Bound by reading the logits once, for which an element must not cost more
+// than a handful of instructions, and by the fixed work of a part (floor,
+// ranking, joining) where there are few rows. The rounds have no barriers.
+//
+// Pooled elements are 64-bit keys, the value's order in the upper half and the
+// complement of the index in the lower, so that no two are equal and the order
+// of threads and blocks decides nothing.
 #ifndef LRRT_PAGED_BEAM_SELECT_CUH_
 #define LRRT_PAGED_BEAM_SELECT_CUH_
 
@@ -17,17 +24,21 @@
 namespace lrrt::ops {
 
 constexpr uint32_t kBeamWarps = kBeamThreads / 32u;
-// Candidates that are ranked against one another at once.
-constexpr uint32_t kBeamPool = 1024;
+constexpr uint32_t kBeamShare = kBeamPool / kBeamWarps; // of the pool, for a warp
+static_assert(kBeamShare == kBeamThreads && kBeamShare >= 2u * kBeamMaximumCount,
+              "a thread takes one key of each share; a share holds the best of two sets");
+
 
 struct BeamShared {
   uint64_t pool[kBeamPool];
-  uint64_t best[kBeamMaximumCount];
-  uint64_t warp_keys[kBeamWarps];
-  float warp_values[kBeamWarps];
-  uint32_t pooled;
+  float noted[kBeamNotedRounds + 1][kBeamThreads]; // maximum of each round and thread
+  uint64_t best[kBeamMaximumCount]; // the pool's best, falling, when it was last ranked
+  uint64_t floors[kBeamWarps][32];
+  float2 sums[kBeamWarps];
+  uint32_t pooled, listed, floor;
   uint32_t last;
 };
+static_assert(sizeof(BeamShared) <= kBeamSharedBytes, "shared memory of a block");
 
 // Order of floats as unsigned numbers; NaN like -infinity.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -43,234 +54,339 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t index) {
   return uint64_t{order_of(x)} << 32 | ~index;
 }
 constexpr uint64_t kNoKey = 0; // below every key
+// What stands for no key in the pool, different at each place: below every
+// key too, whose order is never 0.
+__device__ __forceinline__ uint64_t key_or_place(uint64_t key, uint32_t place) {
+  return key == kNoKey ? uint64_t{place} + 1u : key;
+}
+__device__ __forceinline__ uint64_t key_or_none(uint64_t key) {
+  return key >> 32 != 0 ? key : kNoKey;
+}
 
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
 
-// The `count` largest of the block's keys (Each per thread, in registers),
-// in shared.best, falling; kNoKey where there are fewer.
-//
-// The block's threads are split into `count` rounded up to a power of two
-// groups; the smallest of the groups' maxima is no larger than the count-th
-// largest key, so only keys from there on are candidates: about
-// count * (1 + 1/2 + ... + 1/count) of them when the order is random. They are
-// ranked by counting the larger ones. Where more than kBeamPool pass, the best
-// are taken one after another instead.
-template <int Each>
-__device__ __forceinline__ void block_best(const uint64_t (&keys)[Each], uint32_t count,
-                                           BeamShared &shared) {
+// The threads are split into `count` rounded up to a power of two classes,
+// each spread over the lanes and warps. The smallest of the classes' maxima is
+// no larger than the count-th largest of all elements; about
+// count * (1 + 1/2 + ... + 1/count) of them reach it where their order is
+// random. One barrier.
+template <typename T>
+__device__ __forceinline__ T class_floor(T mine, uint32_t count, BeamShared &shared) {
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5u;
-  uint64_t mine = kNoKey;
+  const bool two = count > 32u; // even and odd warps have classes of their own
+  uint32_t lanes = 1;
+  while (lanes < count && lanes < 32u) {
+    lanes <<= 1u;
+  }
 #pragma unroll
-  for (int i = 0; i < Each; ++i) {
-    mine = larger(mine, keys[i]);
+  for (uint32_t offset = 16; offset != 0; offset >>= 1u) {
+    const T other = __shfl_xor_sync(kAllLanes, mine, offset);
+    mine = offset >= lanes && other > mine ? other : mine;
   }
-  // Groups within a warp: 32 / (groups per warp) lanes each; with no more
-  // groups than warps, whole warps.
-  uint32_t groups = 1;
-  while (groups < count) {
-    groups <<= 1u;
-  }
-  const uint32_t lanes = groups <= kBeamWarps ? 32u : 32u * kBeamWarps / groups;
-  uint64_t group_best = mine;
+  T *floors = reinterpret_cast<T *>(shared.floors);
+  floors[warp * 32u + lane] = mine;
+  __syncthreads();
+  T even = floors[lane], odd = floors[32u + lane];
 #pragma unroll
-  for (uint32_t offset = 1; offset < 32u; offset <<= 1u) {
-    const uint64_t other = __shfl_xor_sync(kAllLanes, group_best, offset);
-    if (offset < lanes) {
-      group_best = larger(group_best, other);
-    }
+  for (uint32_t w = 2; w < kBeamWarps; w += 2u) {
+    const T x = floors[w * 32u + lane], y = floors[(w + 1u) * 32u + lane];
+    even = x > even ? x : even;
+    odd = y > odd ? y : odd;
   }
-  uint64_t floor = group_best; // the smallest of the warp's groups
+  T least = two == (odd < even) ? odd : even; // of two classes the smaller, of one the larger
 #pragma unroll
-  for (uint32_t offset = 1; offset < 32u; offset <<= 1u) {
-    const uint64_t other = __shfl_xor_sync(kAllLanes, floor, offset);
-    floor = floor < other ? floor : other;
+  for (uint32_t offset = 16; offset != 0; offset >>= 1u) {
+    const T other = __shfl_xor_sync(kAllLanes, least, offset);
+    least = other < least ? other : least;
   }
-  __syncthreads(); // shared is free
-  if (lane == 0) {
-    shared.warp_keys[warp] = floor;
-  }
+  return least;
+}
+
+// The count-th largest of the threads' values: about `count` elements of all
+// reach it, and at least that many. Two barriers.
+__device__ __forceinline__ float count_floor(float mine, uint32_t count, BeamShared &shared) {
+  float *values = reinterpret_cast<float *>(shared.floors);
   if (threadIdx.x == 0) {
-    shared.pooled = 0;
+    shared.floor = ~0u;
+  }
+  values[threadIdx.x] = mine;
+  __syncthreads();
+  uint32_t larger_ones = 0;
+#pragma unroll 4
+  for (uint32_t j = 0; j < kBeamThreads / 4u; ++j) {
+    const float4 v = reinterpret_cast<const float4 *>(values)[j];
+    larger_ones += (v.x > mine ? 1u : 0u) + (v.y > mine ? 1u : 0u) + (v.z > mine ? 1u : 0u) +
+                   (v.w > mine ? 1u : 0u);
+  }
+  if (larger_ones < count) {
+    atomicMin(&shared.floor, order_of(mine));
   }
   __syncthreads();
-  floor = shared.warp_keys[0];
+  return value_of(shared.floor);
+}
+
+__device__ __forceinline__ uint64_t warp_largest(uint64_t key) {
 #pragma unroll
-  for (uint32_t w = 1; w < kBeamWarps; ++w) {
-    floor = floor < shared.warp_keys[w] ? floor : shared.warp_keys[w];
+  for (uint32_t offset = 16; offset != 0; offset >>= 1u) {
+    key = larger(key, __shfl_xor_sync(kAllLanes, key, offset));
   }
-  if (mine >= floor) {
-#pragma unroll
-    for (int i = 0; i < Each; ++i) {
-      if (keys[i] >= floor && keys[i] != kNoKey) {
-        const uint32_t at = atomicAdd(&shared.pooled, 1u);
-        if (at < kBeamPool) {
-          shared.pool[at] = keys[i];
-        }
-      }
-    }
-  }
-  if (threadIdx.x < count) {
-    shared.best[threadIdx.x] = kNoKey;
-  }
+  return key;
+}
+
+// Puts the `count` largest of the pool's first `total` keys into `best`, falling,
+// kNoKey after the last: ranked by counting the larger ones; with more keys
+// than threads those below a floor are dropped first, and where that leaves too
+// many to count, the largest are taken one after another. The pool's contents
+// are lost. Begins and ends with a barrier.
+__device__ __noinline__ void rank_pool(uint32_t total, uint32_t count, BeamShared &shared) {
+  constexpr uint32_t kRanked = 1024; // as many are counted against one another
+  const uint32_t thread = threadIdx.x;
   __syncthreads();
-  const uint32_t pooled = shared.pooled;
-  if (pooled <= kBeamPool) {
-    for (uint32_t i = threadIdx.x; i < pooled; i += kBeamThreads) {
-      const uint64_t key = shared.pool[i];
+  if (total <= kBeamThreads) {
+    // One, two or four threads for a key, each counting among as many others.
+    const uint32_t shift = total <= kBeamThreads / 4u ? 2u : total <= kBeamThreads / 2u ? 1u : 0u;
+    const uint32_t parts = 1u << shift, at = thread >> shift;
+    if (at < (total + 7u & ~7u)) { // whole warps
+      const uint64_t key = at < total ? shared.pool[at] : kNoKey;
       uint32_t rank = 0;
-      for (uint32_t j = 0; j < pooled; ++j) {
+#pragma unroll 8
+      for (uint32_t j = thread & (parts - 1u); j < total; j += parts) {
         rank += shared.pool[j] > key ? 1u : 0u;
       }
-      if (rank < count) {
-        shared.best[rank] = key;
+      const unsigned lanes = __activemask();
+      rank += shift > 0u ? __shfl_xor_sync(lanes, rank, 1) : 0u;
+      rank += shift > 1u ? __shfl_xor_sync(lanes, rank, 2) : 0u;
+      if (at < total && rank < count) {
+        shared.best[rank] = key_or_none(key);
       }
+    }
+    if (thread >= total && thread < count) {
+      shared.best[thread] = kNoKey;
     }
     __syncthreads();
     return;
   }
+  uint64_t keys[kBeamWarps];
+  uint64_t mine = kNoKey;
+#pragma unroll
+  for (uint32_t i = 0; i < kBeamWarps; ++i) {
+    const uint32_t at = i * kBeamThreads + thread;
+    keys[i] = at < total ? shared.pool[at] : kNoKey;
+    mine = larger(mine, keys[i]);
+  }
+  if (thread == 0) {
+    shared.pooled = 0;
+  }
+  const uint64_t floor = larger(kNoKey + 1u, class_floor(mine, count, shared));
+  if (mine >= floor) {
+#pragma unroll
+    for (uint32_t i = 0; i < kBeamWarps; ++i) {
+      if (keys[i] >= floor) {
+        shared.pool[atomicAdd(&shared.pooled, 1u)] = keys[i];
+      }
+    }
+  }
+  __syncthreads();
+  total = shared.pooled;
+  if (total <= kRanked) {
+#pragma unroll 1
+    for (uint32_t at = thread; at < total; at += kBeamThreads) {
+      const uint64_t key = shared.pool[at];
+      uint32_t rank = 0;
+#pragma unroll 8
+      for (uint32_t j = 0; j < total; ++j) {
+        rank += shared.pool[j] > key ? 1u : 0u;
+      }
+      if (rank < count) {
+        shared.best[rank] = key_or_none(key);
+      }
+    }
+    if (thread >= total && thread < count) {
+      shared.best[thread] = kNoKey;
+    }
+  } else {
+    uint64_t bound = ~uint64_t{0};
+#pragma unroll 1
+    for (uint32_t rank = 0; rank < count; ++rank) {
+      uint64_t best = kNoKey;
+#pragma unroll
+      for (uint32_t i = 0; i < kBeamWarps; ++i) {
+        best = keys[i] < bound ? larger(best, keys[i]) : best;
+      }
+      best = warp_largest(best);
+      __syncthreads();
+      if ((thread & 31u) == 0) {
+        shared.floors[thread >> 5u][0] = best;
+      }
+      __syncthreads();
+      bound = shared.floors[0][0];
+#pragma unroll
+      for (uint32_t w = 1; w < kBeamWarps; ++w) {
+        bound = larger(bound, shared.floors[w][0]);
+      }
+      if (thread == 0) {
+        shared.best[rank] = key_or_none(bound);
+      }
+    }
+  }
+  __syncthreads();
+}
+
+// The same for one warp's share, which it has alone: one largest after
+// another. Returns the last of them.
+__device__ __noinline__ uint64_t prune_share(uint64_t *share, uint32_t held, uint32_t count) {
+  const uint32_t lane = threadIdx.x & 31u;
+  constexpr uint32_t kEach = kBeamShare / 32u;
+  uint64_t keys[kEach];
+  __syncwarp();
+#pragma unroll
+  for (uint32_t i = 0; i < kEach; ++i) {
+    keys[i] = i * 32u + lane < held ? share[i * 32u + lane] : kNoKey;
+  }
+  __syncwarp();
   uint64_t bound = ~uint64_t{0};
+#pragma unroll 1
   for (uint32_t rank = 0; rank < count; ++rank) {
     uint64_t best = kNoKey;
 #pragma unroll
-    for (int i = 0; i < Each; ++i) {
+    for (uint32_t i = 0; i < kEach; ++i) {
       best = keys[i] < bound ? larger(best, keys[i]) : best;
     }
-#pragma unroll
-    for (uint32_t offset = 16; offset != 0; offset >>= 1u) {
-      best = larger(best, __shfl_xor_sync(kAllLanes, best, offset));
-    }
+    bound = warp_largest(best);
     if (lane == 0) {
-      shared.warp_keys[warp] = best;
-    }
-    __syncthreads();
-    best = shared.warp_keys[0];
-#pragma unroll
-    for (uint32_t w = 1; w < kBeamWarps; ++w) {
-      best = larger(best, shared.warp_keys[w]);
-    }
-    if (threadIdx.x == 0) {
-      shared.best[rank] = best;
-    }
-    bound = best;
-    __syncthreads();
-  }
-}
-
-// As block_best, over `total` keys in global memory, 2048 at a time with the
-// best so far among them.
-__device__ __forceinline__ void block_best_of(const uint64_t *keys, uint32_t total, uint32_t count,
-                                              BeamShared &shared) {
-  constexpr int kEach = 8;
-  constexpr uint32_t kRound = kBeamThreads * kEach;
-  uint32_t done = 0;
-  while (true) {
-    uint64_t held[kEach];
-    const uint32_t kept = done == 0 ? 0u : count;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const uint32_t at = i * kBeamThreads + threadIdx.x;
-      if (at < kept) {
-        held[i] = shared.best[at];
-      } else {
-        const uint64_t from = uint64_t{done} + at - kept;
-        held[i] = from < total ? __ldcg(keys + from) : kNoKey;
-      }
-    }
-    block_best(held, count, shared);
-    done += kRound - kept;
-    if (done >= total) {
-      return;
+      share[rank] = bound;
     }
   }
+  __syncwarp();
+  return bound;
 }
 
-__device__ __forceinline__ float block_max(float x, BeamShared &shared) {
-  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5u;
+// Maximum (times log2 e) and sum of a set of elements, and of two sets.
+__device__ __forceinline__ float2 join_sums(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x);
+  const float base = top == -INFINITY ? 0.0f : top;
+  return make_float2(top, a.y * exp2_fast(a.x - base) + b.y * exp2_fast(b.x - base));
+}
+__device__ __forceinline__ float2 join_lanes(float2 mine) {
 #pragma unroll
   for (uint32_t offset = 16; offset != 0; offset >>= 1u) {
-    x = fmaxf(x, __shfl_xor_sync(kAllLanes, x, offset));
+    mine = join_sums(mine, make_float2(__shfl_xor_sync(kAllLanes, mine.x, offset),
+                                       __shfl_xor_sync(kAllLanes, mine.y, offset)));
   }
-  __syncthreads();
-  if (lane == 0) {
-    shared.warp_values[warp] = x;
-  }
-  __syncthreads();
-  x = shared.warp_values[0];
-#pragma unroll
-  for (uint32_t w = 1; w < kBeamWarps; ++w) {
-    x = fmaxf(x, shared.warp_values[w]);
-  }
-  return x;
+  return mine;
 }
 
-__device__ __forceinline__ float block_sum(float x, BeamShared &shared) {
-  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5u;
-#pragma unroll
-  for (uint32_t offset = 16; offset != 0; offset >>= 1u) {
-    x += __shfl_xor_sync(kAllLanes, x, offset);
+// Elements in 32-bit words: their values, the larger of two words element by
+// element (NaN only where both are), and the largest of a word's.
+template <typename T> struct Words;
+template <> struct Words<float> {
+  static constexpr uint32_t kLeast = 0xff800000u; // -infinity
+  static __device__ __forceinline__ void set(uint32_t &word, int, float x) {
+    word = __float_as_uint(x);
   }
-  __syncthreads();
-  if (lane == 0) {
-    shared.warp_values[warp] = x;
+  static __device__ __forceinline__ float value(uint32_t word, int) {
+    return __uint_as_float(word);
   }
-  __syncthreads();
-  x = shared.warp_values[0];
-#pragma unroll
-  for (uint32_t w = 1; w < kBeamWarps; ++w) {
-    x += shared.warp_values[w];
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
   }
-  return x;
-}
+  static __device__ __forceinline__ float largest(uint32_t word) { return __uint_as_float(word); }
+};
+template <> struct Words<__nv_bfloat16> {
+  static constexpr uint32_t kLeast = 0xff80ff80u; // -infinity
+  static __device__ __forceinline__ void set(uint32_t &word, int half, __nv_bfloat16 x) {
+    uint16_t bits;
+    memcpy(&bits, &x, 2);
+    word = half == 0 ? (word & 0xffff0000u) | bits : (word & 0xffffu) | uint32_t{bits} << 16;
+  }
+  static __device__ __forceinline__ float value(uint32_t word, int half) {
+    return __uint_as_float(half == 0 ? word << 16 : word & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    __nv_bfloat162 x, y;
+    memcpy(&x, &a, 4);
+    memcpy(&y, &b, 4);
+    x = __hmax2(x, y);
+    memcpy(&a, &x, 4);
+    return a;
+  }
+  static __device__ __forceinline__ float largest(uint32_t word) {
+    return fmaxf(value(word, 0), value(word, 1));
+  }
+};
+template <> struct Words<__half> {
+  static constexpr uint32_t kLeast = 0xfc00fc00u; // -infinity
+  static __device__ __forceinline__ void set(uint32_t &word, int half, __half x) {
+    uint16_t bits;
+    memcpy(&bits, &x, 2);
+    word = half == 0 ? (word & 0xffff0000u) | bits : (word & 0xffffu) | uint32_t{bits} << 16;
+  }
+  static __device__ __forceinline__ float value(uint32_t word, int half) {
+    __half2 x;
+    memcpy(&x, &word, 4);
+    return half == 0 ? __low2float(x) : __high2float(x);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    __half2 x, y;
+    memcpy(&x, &a, 4);
+    memcpy(&y, &b, 4);
+    x = __hmax2(x, y);
+    memcpy(&a, &x, 4);
+    return a;
+  }
+  static __device__ __forceinline__ float largest(uint32_t word) {
+    return fmaxf(value(word, 0), value(word, 1));
+  }
+};
 
 // Whether this block is the last of `blocks` to get here; its reads then see
 // what the others wrote before. The counter is zero again afterwards.
 __device__ __forceinline__ bool arrive_last(uint32_t *counter, uint32_t blocks,
                                             BeamShared &shared) {
-  __threadfence();
+  if (blocks == 1u) {
+    __syncthreads();
+    return true;
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
+    __threadfence(); // what the barrier showed this thread, to the whole GPU
     const uint32_t before = atomicAdd(counter, 1u);
     shared.last = before + 1u == blocks ? 1u : 0u;
     if (shared.last != 0) {
       *counter = 0;
     }
+    __threadfence();
   }
   __syncthreads();
-  __threadfence();
   return shared.last != 0;
 }
 
 // The beams of a group against one another.
 __device__ __forceinline__ void rank_beams(const BeamArgs &args, uint32_t group,
                                            BeamShared &shared) {
-  constexpr int kEach = kBeamMaximumCandidates / kBeamThreads;
   const uint32_t candidates = args.beams * args.count;
-  uint64_t keys[kEach];
-#pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    const uint32_t at = i * kBeamThreads + threadIdx.x;
-    keys[i] = kNoKey;
-    if (at < candidates) {
-      const uint32_t beam = at / args.count, rank = at - beam * args.count;
-      const uint32_t row = group * args.beams + beam;
-      float score = args.scores[row];
-      if (args.finished == nullptr || args.finished[row] == 0) {
-        const uint64_t key = __ldcg(args.row_keys + uint64_t{row} * args.count + rank);
-        const float logit = value_of(static_cast<uint32_t>(key >> 32));
-        score = key == kNoKey ? -INFINITY : score + (logit - __ldcg(args.row_log_sums + row));
-      } else if (rank != 0) {
-        score = -INFINITY;
-      }
-      keys[i] = score > -INFINITY ? key_of(score, at) : kNoKey; // NaN: no candidate
+#pragma unroll 1
+  for (uint32_t at = threadIdx.x; at < candidates; at += kBeamThreads) {
+    const uint32_t beam = at / args.count, rank = at - beam * args.count;
+    const uint32_t row = group * args.beams + beam;
+    float score = args.scores[row];
+    if (args.finished == nullptr || args.finished[row] == 0) {
+      const uint64_t key = __ldcg(args.row_keys + uint64_t{row} * args.count + rank);
+      const float logit = value_of(static_cast<uint32_t>(key >> 32));
+      score = key == kNoKey ? -INFINITY : score + (logit - __ldcg(args.row_log_sums + row));
+    } else if (rank != 0) {
+      score = -INFINITY;
     }
+    const uint64_t key = score > -INFINITY ? key_of(score, at) : kNoKey; // NaN: no candidate
+    shared.pool[at] = key_or_place(key, at);
   }
-  block_best(keys, args.count, shared);
+  rank_pool(candidates, args.count, shared);
+  bool finished = true;
+  const uint64_t out = uint64_t{group} * args.count + threadIdx.x;
   if (threadIdx.x < args.count) {
     const uint64_t key = shared.best[threadIdx.x];
-    const uint64_t out = uint64_t{group} * args.count + threadIdx.x;
     float score = -INFINITY;
     int32_t parent = -1, token = -1;
-    bool finished = true;
     if (key != kNoKey) {
       const uint32_t at = ~static_cast<uint32_t>(key);
       const uint32_t beam = at / args.count, rank = at - beam * args.count;
@@ -286,102 +402,263 @@ __device__ __forceinline__ void rank_beams(const BeamArgs &args, uint32_t group,
         finished = token == args.end_token;
       }
     }
-    shared.pool[threadIdx.x] = uint64_t{finished ? 1u : 0u};
     args.parents_out[out] = parent;
     args.tokens_out[out] = token;
-    // scores_out may be scores: all of the group's were read before the
-    // barriers above; finished_out is stored behind one more.
-    args.scores_out[out] = score;
+    args.scores_out[out] = score; // may be `scores`: all were read before the barriers above
   }
-  __syncthreads();
+  __syncthreads(); // finished_out may be `finished`
   if (threadIdx.x < args.count && args.finished_out != nullptr) {
-    args.finished_out[uint64_t{group} * args.count + threadIdx.x] =
-        static_cast<uint8_t>(shared.pool[threadIdx.x]);
+    args.finished_out[out] = finished ? 1u : 0u;
   }
 }
 
-// grid (chunks, rows). Width elements a load, Loads of them per thread.
-template <typename T, int Width, int Loads>
+// grid (parts, rows). Width elements a load.
+template <typename T, int Width>
 __device__ __forceinline__ void beam_select(const BeamArgs &args) {
-  __shared__ BeamShared shared;
-  constexpr int kEach = Width * Loads;
-  constexpr uint32_t kChunk = kBeamThreads * kEach;
-  const uint32_t chunk = blockIdx.x, row = blockIdx.y;
+  extern __shared__ __align__(16) unsigned char beam_memory[];
+  BeamShared &shared = *reinterpret_cast<BeamShared *>(beam_memory);
+  constexpr uint32_t kRound = beam_round(sizeof(T));
+  constexpr int kEach = kRound / kBeamThreads; // elements of a thread and round
+  constexpr int kPerWord = 4 / sizeof(T);
+  constexpr int kWords = kEach / kPerWord;
+  using W = Words<T>;
+  const uint32_t part = blockIdx.x, row = blockIdx.y;
   const uint32_t group = row / args.beams;
+  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5u;
   const bool going = args.finished == nullptr || args.finished[row] == 0;
   if (going) {
     const T *logits = static_cast<const T *>(args.logits) + row * args.logits_stride;
-    const uint32_t begin = chunk * kChunk;
-    float x[kEach];
+    const uint32_t begin = part * args.part_elements;
+    const uint32_t end = min(args.vocab, begin + args.part_elements);
+    auto index_of = [&](uint32_t round, int i) {
+      return round + ((i / Width) * kBeamThreads + threadIdx.x) * Width + i % Width;
+    };
+    // A thread's elements of a round, -infinity past the last whole vector.
+    const uint32_t whole = end - (end - begin) % Width;
+    auto load = [&](uint32_t(&to)[kWords], uint32_t round) {
 #pragma unroll
-    for (int load = 0; load < Loads; ++load) {
-      const uint32_t at = begin + (load * kBeamThreads + threadIdx.x) * Width;
-      if (at + Width <= args.vocab) {
-        const auto v = *reinterpret_cast<const Vector<T, Width> *>(logits + at);
+      for (int k = 0; k < kWords; ++k) {
+        to[k] = W::kLeast;
+      }
 #pragma unroll
-        for (int i = 0; i < Width; ++i) {
-          x[load * Width + i] = to_float(v.at[i]);
+      for (int i = 0; i < kEach; i += Width) {
+        const uint32_t index = index_of(round, i);
+        if (index < whole) {
+          if constexpr (Width == 1) {
+            W::set(to[i / kPerWord], i % kPerWord, logits[index]);
+          } else {
+            const uint4 v = *reinterpret_cast<const uint4 *>(logits + index);
+            to[i / kPerWord] = v.x;
+            to[i / kPerWord + 1] = v.y;
+            to[i / kPerWord + 2] = v.z;
+            to[i / kPerWord + 3] = v.w;
+          }
         }
-      } else {
+      }
+    };
+    float top = -INFINITY, sum = 0.0f; // as join_sums takes them
+    float largest = -INFINITY;
+    auto take = [&](const uint32_t(&from)[kWords], uint32_t round, uint32_t number) {
+      uint32_t larger_word = from[0];
 #pragma unroll
-        for (int i = 0; i < Width; ++i) {
-          x[load * Width + i] = at + i < args.vocab ? to_float(logits[at + i]) : -INFINITY;
+      for (int k = 1; k < kWords; ++k) {
+        larger_word = W::larger(larger_word, from[k]);
+      }
+      const float most = fmaxf(W::largest(larger_word), -INFINITY); // NaN counts as -infinity
+      shared.noted[number][threadIdx.x] = most;
+      largest = fmaxf(largest, most);
+      const float now = fmaxf(top, most * kLog2E);
+      const float base = now == -INFINITY ? 0.0f : now;
+      float terms = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        terms += exp2_fast(fmaf(W::value(from[i / kPerWord], i % kPerWord), kLog2E, -base));
+      }
+      if (terms != terms) { // there is a NaN
+        terms = 0.0f;
+#pragma unroll 1
+        for (int i = 0; i < kEach; ++i) {
+          const uint32_t index = index_of(round, i);
+          const float y = index < whole ? to_float(logits[index]) : -INFINITY;
+          terms += y == y ? exp2_fast(fmaf(y, kLog2E, -base)) : 0.0f;
+        }
+      }
+      sum = sum * exp2_fast(top - base) + terms;
+      top = now;
+    };
+    // Two rounds are under way: a buffer is filled again once it is used up.
+    constexpr uint32_t kAhead = 2;
+    uint32_t buffers[kAhead][kWords];
+    const uint32_t rounds = (whole - begin + kRound - 1u) / kRound;
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead; ++i) {
+      if (i < rounds) {
+        load(buffers[i], begin + i * kRound);
+      }
+    }
+#pragma unroll 1
+    for (uint32_t number = 0; number < rounds; number += kAhead) {
+#pragma unroll
+      for (uint32_t i = 0; i < kAhead; ++i) {
+        if (number + i < rounds) {
+          const uint32_t round = begin + (number + i) * kRound;
+          take(buffers[i], round, number + i);
+          if (number + i + kAhead < rounds) {
+            load(buffers[i], round + kAhead * kRound);
+          }
         }
       }
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      top = fmaxf(top, x[i]); // passes over NaN
+
+    // Elements past the last whole vector: one more round, of an element for
+    // each of the first threads.
+    float odd = -INFINITY;
+    if (Width > 1 && threadIdx.x < end - whole) {
+      odd = to_float(logits[whole + threadIdx.x]);
+      odd = odd == odd ? odd : -INFINITY;
+      largest = fmaxf(largest, odd);
+      const float2 joined = join_sums(make_float2(top, sum), make_float2(odd * kLog2E, 1.0f));
+      top = joined.x;
+      sum = joined.y;
     }
-    top = block_max(top, shared);
-    const float base = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const float e = exp2_fast((x[i] - base) * kLog2E);
-      sum += x[i] != x[i] ? 0.0f : e;
+    shared.noted[rounds][threadIdx.x] = odd;
+
+    // What reaches the floor, into the pool: rounds of threads with such a
+    // maximum are listed, and each is read again by a warp, an element a lane,
+    // four such reads at a time.
+    static_assert(kEach <= 32, "a lane per element");
+    static_assert((kBeamNotedRounds + 1u) * kBeamThreads <= 65536u, "a listed round is 16 bits");
+    constexpr uint32_t kListed = 2u * kBeamPool, kPooled = kBeamPool / 2u;
+    auto *list = reinterpret_cast<uint16_t *>(shared.pool + kPooled); // the pool's other half
+    if (threadIdx.x == 0) {
+      shared.pooled = 0;
+      shared.listed = 0;
     }
-    sum = block_sum(sum, shared);
-    uint64_t keys[kEach];
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const uint32_t at = begin + ((i / Width) * kBeamThreads + threadIdx.x) * Width + i % Width;
-      keys[i] = at < args.vocab ? key_of(x[i], at) : kNoKey;
+    float floor = count_floor(largest, args.count, shared);
+    uint64_t least_key = uint64_t{order_of(floor)} << 32; // the lowest that enters
+#pragma unroll 4
+    for (uint32_t i = 0; i <= rounds; ++i) {
+      if (shared.noted[i][threadIdx.x] >= floor) {
+        const uint32_t at = atomicAdd(&shared.listed, 1u);
+        if (at < kListed) {
+          list[at] = static_cast<uint16_t>(i * kBeamThreads + threadIdx.x);
+        }
+      }
     }
-    block_best(keys, args.count, shared);
-    const uint64_t slot = uint64_t{row} * args.chunks + chunk;
-    if (threadIdx.x < args.count) {
-      args.chunk_keys[slot * args.count + threadIdx.x] = shared.best[threadIdx.x];
+    __syncthreads();
+    // The key of this lane's element of a thread's round.
+    auto key_at = [&](uint32_t i, uint32_t thread) -> uint64_t {
+      uint32_t index =
+          begin + i * kRound + (lane / Width * kBeamThreads + thread) * Width + lane % Width;
+      bool there = lane < kEach && index < whole;
+      if (i == rounds) {
+        index = whole + thread;
+        there = lane == 0 && index < end;
+      }
+      return there ? key_of(to_float(logits[index]), index) : kNoKey;
+    };
+    const uint32_t listed = shared.listed;
+#pragma unroll 1
+    for (uint32_t first = warp; first < min(listed, kListed); first += 4u * kBeamWarps) {
+      uint64_t keys[4];
+#pragma unroll
+      for (uint32_t k = 0; k < 4u; ++k) {
+        const uint32_t at = first + k * kBeamWarps;
+        keys[k] = kNoKey;
+        if (at < min(listed, kListed)) {
+          keys[k] = key_at(list[at] / kBeamThreads, list[at] % kBeamThreads);
+        }
+      }
+#pragma unroll
+      for (uint32_t k = 0; k < 4u; ++k) {
+        if (keys[k] >= least_key) {
+          const uint32_t at = atomicAdd(&shared.pooled, 1u);
+          if (at < kPooled) {
+            shared.pool[at] = keys[k];
+          }
+        }
+      }
+    }
+    __syncthreads();
+    uint32_t total = shared.pooled;
+    if (listed > kListed || total > kPooled) {
+      // Equal values, or an order that defeats the floor: each warp keeps the
+      // best of its threads' elements in its share of the pool, raising the
+      // floor as it goes.
+      __syncthreads();
+      uint64_t *share = shared.pool + warp * kBeamShare;
+      uint32_t held = 0;
+#pragma unroll 1
+      for (uint32_t i = 0; i <= rounds; ++i) {
+        uint32_t looking = __ballot_sync(kAllLanes, shared.noted[i][threadIdx.x] >= floor);
+#pragma unroll 1
+        for (; looking != 0; looking &= looking - 1u) {
+          const uint64_t key = key_at(i, warp * 32u + __ffs(looking) - 1u);
+          const uint32_t entering = __ballot_sync(kAllLanes, key >= least_key);
+          if (key >= least_key) {
+            share[held + __popc(entering & ((1u << lane) - 1u))] = key;
+          }
+          held += __popc(entering);
+          if (held + 32u > kBeamShare) {
+            least_key = prune_share(share, held, args.count) + 1u;
+            held = args.count;
+            floor = value_of(static_cast<uint32_t>(least_key >> 32));
+          }
+        }
+      }
+      for (uint32_t at = held + lane; at < kBeamShare; at += 32u) {
+        share[at] = key_or_place(kNoKey, warp * kBeamShare + at);
+      }
+      total = kBeamPool;
+    }
+    const float2 sums = join_lanes(make_float2(top, sum));
+    if (lane == 0) {
+      shared.sums[warp] = sums;
+    }
+    rank_pool(total, args.count, shared);
+    const uint64_t slot = uint64_t{row} * args.parts + part;
+    if (args.parts != 1u && threadIdx.x < args.count) {
+      args.part_keys[slot * args.count + threadIdx.x] = shared.best[threadIdx.x];
     }
     if (threadIdx.x == 0) {
-      args.chunk_sums[slot] = {top, sum};
+      float2 all = shared.sums[0];
+#pragma unroll
+      for (uint32_t w = 1; w < kBeamWarps; ++w) {
+        all = join_sums(all, shared.sums[w]);
+      }
+      if (args.parts != 1u) {
+        args.part_sums[slot] = {all.x, all.y};
+      } else {
+        args.row_log_sums[row] = (all.x + log2f(all.y)) * kLn2;
+      }
     }
   }
-  if (!arrive_last(args.row_arrivals + row, args.chunks, shared)) {
+  if (!arrive_last(args.row_arrivals + row, args.parts, shared)) {
     return;
   }
   if (going) {
-    const auto *sums =
-        reinterpret_cast<const float2 *>(args.chunk_sums + uint64_t{row} * args.chunks);
-    float top = -INFINITY;
-    for (uint32_t i = threadIdx.x; i < args.chunks; i += kBeamThreads) {
-      top = fmaxf(top, __ldcg(sums + i).x);
+    if (args.parts != 1u) {
+      const uint64_t *keys = args.part_keys + uint64_t{row} * args.parts * args.count;
+      const uint32_t total = args.parts * args.count;
+#pragma unroll 2
+      for (uint32_t at = threadIdx.x; at < total; at += kBeamThreads) {
+        shared.pool[at] = key_or_place(__ldcg(keys + at), at);
+      }
+      if (warp == kBeamWarps - 1u) { // the last one: it has the fewest keys to bring
+        const auto *sums =
+            reinterpret_cast<const float2 *>(args.part_sums) + uint64_t{row} * args.parts;
+        const float2 none = make_float2(-INFINITY, 0.0f);
+        const float2 all =
+            join_lanes(join_sums(lane < args.parts ? __ldcg(sums + lane) : none,
+                                 lane + 32u < args.parts ? __ldcg(sums + lane + 32u) : none));
+        if (lane == 0) {
+          args.row_log_sums[row] = (all.x + log2f(all.y)) * kLn2;
+        }
+      }
+      rank_pool(total, args.count, shared);
     }
-    top = block_max(top, shared);
-    float sum = 0.0f;
-    for (uint32_t i = threadIdx.x; i < args.chunks; i += kBeamThreads) {
-      const float2 s = __ldcg(sums + i);
-      sum += s.x == -INFINITY ? 0.0f : s.y * exp2_fast((s.x - top) * kLog2E);
-    }
-    sum = block_sum(sum, shared);
-    block_best_of(args.chunk_keys + uint64_t{row} * args.chunks * args.count,
-                  args.chunks * args.count, args.count, shared);
     if (threadIdx.x < args.count) {
       args.row_keys[uint64_t{row} * args.count + threadIdx.x] = shared.best[threadIdx.x];
-    }
-    if (threadIdx.x == 0) {
-      args.row_log_sums[row] = top + logf(sum);
     }
   }
   if (!arrive_last(args.group_arrivals + group, args.beams, shared)) {

@@ -471,7 +471,7 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
   require(a.beams >= 1 && a.beams <= kBeamMaximumCount && a.count >= 1 &&
               a.count <= kBeamMaximumCount && a.beams * a.count <= kBeamMaximumCandidates,
           "beams and count must be 1 to 64, their product at most 2048");
-  require(a.vocab >= a.count && a.vocab <= 0x7fffffffu, "vocab must be count to 2^31 - 1");
+  require(a.vocab >= a.count && a.vocab <= kBeamMaximumVocab, "vocab must be count to 2^21");
   require(uint64_t{a.groups} * a.beams <= 65535u, "at most 65535 beams in all");
   if (a.groups == 0) {
     return;
@@ -488,9 +488,24 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
   const bool wide = multiple_of(a.logits, 16) && multiple_of(a.logits_row_stride, element, 16);
   const uint32_t width = wide ? static_cast<uint32_t>(16u / element) : 1u;
   const size_t rows = size_t{a.groups} * a.beams;
-  const size_t chunks = ceil_div(a.vocab, kBeamThreads * 16u);
-  const size_t sums_at = aligned(8u * rows * chunks * a.count),
-               row_keys_at = sums_at + aligned(8u * rows * chunks),
+  // Parts of a row: the SM with most of them reads so many rounds one after
+  // another, and joining several parts takes about as long as eight.
+  const uint32_t round = beam_round(static_cast<uint32_t>(element));
+  const uint64_t rounds = ceil_div(a.vocab, round);
+  const uint64_t most = std::min<uint64_t>({rounds, kBeamMaximumParts, kBeamPool / a.count});
+  uint64_t parts = 1, least = ~uint64_t{0};
+  for (uint64_t n = ceil_div(rounds, kBeamNotedRounds); n <= most; ++n) {
+    const uint64_t cost =
+        ceil_div(rows * n, context.sms) * ceil_div(rounds, n) + (n > 1u ? 8u : 0u);
+    if (cost < least) {
+      least = cost;
+      parts = n;
+    }
+  }
+  const uint64_t part_elements = (ceil_div(a.vocab, parts) + 7u) / 8u * 8u;
+  parts = ceil_div(a.vocab, part_elements);
+  const size_t sums_at = aligned(8u * rows * parts * a.count),
+               row_keys_at = sums_at + aligned(8u * rows * parts),
                log_sums_at = row_keys_at + aligned(8u * rows * a.count);
   context.reserve(log_sums_at + aligned(4u * rows));
   context.reserve_counters(rows + a.groups);
@@ -509,16 +524,17 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
   args.beams = a.beams;
   args.vocab = a.vocab;
   args.count = a.count;
-  args.chunks = static_cast<uint32_t>(chunks);
+  args.parts = static_cast<uint32_t>(parts);
+  args.part_elements = static_cast<uint32_t>(part_elements);
   args.end_token = a.end_token;
-  args.chunk_keys = reinterpret_cast<uint64_t *>(scratch);
-  args.chunk_sums = reinterpret_cast<Pair *>(scratch + sums_at);
+  args.part_keys = reinterpret_cast<uint64_t *>(scratch);
+  args.part_sums = reinterpret_cast<Pair *>(scratch + sums_at);
   args.row_keys = reinterpret_cast<uint64_t *>(scratch + row_keys_at);
   args.row_log_sums = reinterpret_cast<float *>(scratch + log_sums_at);
   args.row_arrivals = counters;
   args.group_arrivals = counters + rows;
   context.launch(std::string("ops_beam_") + type_name(a.type) + "_x" + std::to_string(width),
-                 chunks, kBeamThreads, 0, args, static_cast<uint32_t>(rows));
+                 parts, kBeamThreads, kBeamSharedBytes, args, static_cast<uint32_t>(rows));
 }
 
 } // namespace
