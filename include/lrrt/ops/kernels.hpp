@@ -42,15 +42,29 @@ struct Divider {
   }
 };
 
+// Strides are in elements and below 2^31, so that an offset is one 32-bit by
+// 32-bit product of 64 bits.
 struct Rows {
   void *data;
-  int64_t row_stride, head_stride; // elements
+  int32_t row_stride, head_stride;
+
+  LRRT_OPS_HD int64_t offset(uint32_t row, uint32_t head) const {
+    return int64_t{row} * row_stride + int64_t{head} * head_stride;
+  }
+};
+
+struct Pages {
+  void *data;
+  int32_t page_stride, token_stride, head_stride;
+
+  LRRT_OPS_HD int64_t offset(uint32_t page, uint32_t token, uint32_t head) const {
+    return int64_t{page} * page_stride + int64_t{token} * token_stride +
+           int64_t{head} * head_stride;
+  }
 };
 
 struct Cache {
-  void *keys, *values;
-  int64_t key_page, key_token, key_head; // strides, elements
-  int64_t value_page, value_token, value_head;
+  Pages keys, values;
   uint32_t page_count, kv_heads;
   Divider page;
 };
@@ -69,12 +83,10 @@ struct RopeAppendArgs {
   Table table;
   const int32_t *sequences, *positions;
   const float *cos_table, *sin_table;
-  uint64_t items; // tokens * items_per_token
-  uint32_t heads, head_dim, rotary_dim, table_positions;
-  // One item is a vector of `width` elements of a head that is copied, or a
-  // vector of each half of its pairs that is rotated.
-  uint32_t items_per_token, turned_items; // turned: those of the q and k heads
-  Divider per_token, per_head, per_value_head;
+  uint32_t items, value_items; // of all tokens' query and key heads, and value heads
+  uint32_t heads, rotary_dim, table_positions;
+  Divider per_token, per_head;             // items of a token, of a head
+  Divider values_per_token, values_per_head;
 };
 
 // Shared memory of an attention block: a ring of tiles for each of its warps,

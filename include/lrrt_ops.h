@@ -17,8 +17,8 @@
  * layer; a sequence's token j is row j % page_size of page
  * table[sequence][j / page_size]. Strides are given in elements, so pages may
  * be stored token by token or head by head; the head_dim elements of one row
- * are contiguous. A table entry outside [0, page_count) is "no page": its
- * tokens are not read and not written.
+ * are contiguous. Strides are less than 2^31 elements. A table entry outside
+ * [0, page_count) is "no page": its tokens are not read and not written.
  *
  * Calls enqueue their work on the context's queue and return; the device
  * arrays they are given must stay until it is done. The calls of one context

@@ -242,11 +242,10 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     if (lane_ == 0) {
       seen_[stage] = seen;
     }
-    const int64_t page = present ? gather.page : 0; // nothing is read there, zeros are written
-    const T *key = static_cast<const T *>(args_.cache.keys) + page * args_.cache.key_page +
-                   gather.row * args_.cache.key_token + gather.head * args_.cache.key_head;
-    const T *value = static_cast<const T *>(args_.cache.values) + page * args_.cache.value_page +
-                     gather.row * args_.cache.value_token + gather.head * args_.cache.value_head;
+    const uint32_t page = present ? gather.page : 0u; // nothing is read there, zeros are written
+    const Pages &k = args_.cache.keys, &v = args_.cache.values;
+    const T *key = static_cast<const T *>(k.data) + k.offset(page, gather.row, gather.head);
+    const T *value = static_cast<const T *>(v.data) + v.offset(page, gather.row, gather.head);
     const uint32_t chunk = lane_ % kChunks;
     const bool inside = chunk * (16u / sizeof(T)) < args_.head_dim;
     const uint32_t offset = inside ? chunk * 16u : 0u;
@@ -274,8 +273,8 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
 #pragma unroll
     for (int n = 0; n < HeadTiles; ++n) {
       const uint32_t head = n * 8u + lane_ / 4u;
-      const T *q = static_cast<const T *>(args_.q.data) + sequence * args_.q.row_stride +
-                   (first_head + min(head, heads - 1u)) * args_.q.head_stride;
+      const T *q = static_cast<const T *>(args_.q.data) +
+                   args_.q.offset(sequence, first_head + min(head, heads - 1u));
       const uint32_t limit = head < heads ? args_.head_dim : 0u;
 #pragma unroll
       for (uint32_t k = 0; k < kSteps; ++k) {
@@ -555,8 +554,8 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
         }
         const float top = maximum_[n][i];
         const float inverse = top == -INFINITY ? 0.0f : 1.0f / sum_[n][i];
-        T *out = static_cast<T *>(args_.out.data) + sequence * args_.out.row_stride +
-                 (first_head + head) * args_.out.head_stride;
+        T *out = static_cast<T *>(args_.out.data) +
+                 args_.out.offset(sequence, first_head + head);
 #pragma unroll
         for (uint32_t d = 0; d < Dim / 16u; ++d) {
 #pragma unroll
@@ -616,8 +615,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
   __device__ __forceinline__ void finish(uint32_t sequence, uint32_t head, uint32_t column,
                                          const Joined &joined) const {
     const float inverse = joined.top == -INFINITY ? 0.0f : 1.0f / joined.sum;
-    T *out = static_cast<T *>(args_.out.data) + sequence * args_.out.row_stride +
-             head * args_.out.head_stride;
+    T *out = static_cast<T *>(args_.out.data) + args_.out.offset(sequence, head);
     const float x[4] = {joined.x.x, joined.x.y, joined.x.z, joined.x.w};
 #pragma unroll
     for (uint32_t i = 0; i < 4u; ++i) {

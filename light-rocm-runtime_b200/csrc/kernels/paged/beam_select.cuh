@@ -276,69 +276,6 @@ __device__ __forceinline__ float2 join_lanes(float2 mine) {
   return mine;
 }
 
-// Elements in 32-bit words: their values, the larger of two words element by
-// element (NaN only where both are), and the largest of a word's.
-template <typename T> struct Words;
-template <> struct Words<float> {
-  static constexpr uint32_t kLeast = 0xff800000u; // -infinity
-  static __device__ __forceinline__ void set(uint32_t &word, int, float x) {
-    word = __float_as_uint(x);
-  }
-  static __device__ __forceinline__ float value(uint32_t word, int) {
-    return __uint_as_float(word);
-  }
-  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
-    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
-  }
-  static __device__ __forceinline__ float largest(uint32_t word) { return __uint_as_float(word); }
-};
-template <> struct Words<__nv_bfloat16> {
-  static constexpr uint32_t kLeast = 0xff80ff80u; // -infinity
-  static __device__ __forceinline__ void set(uint32_t &word, int half, __nv_bfloat16 x) {
-    uint16_t bits;
-    memcpy(&bits, &x, 2);
-    word = half == 0 ? (word & 0xffff0000u) | bits : (word & 0xffffu) | uint32_t{bits} << 16;
-  }
-  static __device__ __forceinline__ float value(uint32_t word, int half) {
-    return __uint_as_float(half == 0 ? word << 16 : word & 0xffff0000u);
-  }
-  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
-    __nv_bfloat162 x, y;
-    memcpy(&x, &a, 4);
-    memcpy(&y, &b, 4);
-    x = __hmax2(x, y);
-    memcpy(&a, &x, 4);
-    return a;
-  }
-  static __device__ __forceinline__ float largest(uint32_t word) {
-    return fmaxf(value(word, 0), value(word, 1));
-  }
-};
-template <> struct Words<__half> {
-  static constexpr uint32_t kLeast = 0xfc00fc00u; // -infinity
-  static __device__ __forceinline__ void set(uint32_t &word, int half, __half x) {
-    uint16_t bits;
-    memcpy(&bits, &x, 2);
-    word = half == 0 ? (word & 0xffff0000u) | bits : (word & 0xffffu) | uint32_t{bits} << 16;
-  }
-  static __device__ __forceinline__ float value(uint32_t word, int half) {
-    __half2 x;
-    memcpy(&x, &word, 4);
-    return half == 0 ? __low2float(x) : __high2float(x);
-  }
-  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
-    __half2 x, y;
-    memcpy(&x, &a, 4);
-    memcpy(&y, &b, 4);
-    x = __hmax2(x, y);
-    memcpy(&a, &x, 4);
-    return a;
-  }
-  static __device__ __forceinline__ float largest(uint32_t word) {
-    return fmaxf(value(word, 0), value(word, 1));
-  }
-};
-
 // Whether this block is the last of `blocks` to get here; its reads then see
 // what the others wrote before. The counter is zero again afterwards.
 __device__ __forceinline__ bool arrive_last(uint32_t *counter, uint32_t blocks,

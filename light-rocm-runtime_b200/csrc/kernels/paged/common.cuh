@@ -32,9 +32,118 @@ template <> __device__ __forceinline__ __half from_float<__half>(float x) {
   return __float2half_rn(x);
 }
 
-// `Count` elements moved as one load or store of at most 16 bytes.
-template <typename T, int Count> struct alignas(sizeof(T) * Count) Vector {
-  T at[Count];
+// Elements in 32-bit words, one or two: their values, words of values (rounded
+// to nearest), the larger of two words element by element (NaN only where both
+// are), and the largest of a word's.
+template <typename T> struct Words;
+template <> struct Words<float> {
+  static constexpr uint32_t kLeast = 0xff800000u; // -infinity
+  static __device__ __forceinline__ uint32_t of(float x, float) { return __float_as_uint(x); }
+  static __device__ __forceinline__ void set(uint32_t &word, int, float x) {
+    word = __float_as_uint(x);
+  }
+  static __device__ __forceinline__ float value(uint32_t word, int) {
+    return __uint_as_float(word);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
+  static __device__ __forceinline__ float largest(uint32_t word) { return __uint_as_float(word); }
+};
+template <> struct Words<__nv_bfloat16> {
+  static constexpr uint32_t kLeast = 0xff80ff80u; // -infinity
+  static __device__ __forceinline__ uint32_t of(float low, float high) {
+    const auto pair = __floats2bfloat162_rn(low, high);
+    uint32_t word;
+    memcpy(&word, &pair, 4);
+    return word;
+  }
+  static __device__ __forceinline__ void set(uint32_t &word, int half, __nv_bfloat16 x) {
+    uint16_t bits;
+    memcpy(&bits, &x, 2);
+    word = half == 0 ? (word & 0xffff0000u) | bits : (word & 0xffffu) | uint32_t{bits} << 16;
+  }
+  static __device__ __forceinline__ float value(uint32_t word, int half) {
+    return __uint_as_float(half == 0 ? word << 16 : word & 0xffff0000u);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    __nv_bfloat162 x, y;
+    memcpy(&x, &a, 4);
+    memcpy(&y, &b, 4);
+    x = __hmax2(x, y);
+    memcpy(&a, &x, 4);
+    return a;
+  }
+  static __device__ __forceinline__ float largest(uint32_t word) {
+    return fmaxf(value(word, 0), value(word, 1));
+  }
+};
+template <> struct Words<__half> {
+  static constexpr uint32_t kLeast = 0xfc00fc00u; // -infinity
+  static __device__ __forceinline__ uint32_t of(float low, float high) {
+    const auto pair = __floats2half2_rn(low, high);
+    uint32_t word;
+    memcpy(&word, &pair, 4);
+    return word;
+  }
+  static __device__ __forceinline__ void set(uint32_t &word, int half, __half x) {
+    uint16_t bits;
+    memcpy(&bits, &x, 2);
+    word = half == 0 ? (word & 0xffff0000u) | bits : (word & 0xffffu) | uint32_t{bits} << 16;
+  }
+  static __device__ __forceinline__ float value(uint32_t word, int half) {
+    __half2 x;
+    memcpy(&x, &word, 4);
+    return half == 0 ? __low2float(x) : __high2float(x);
+  }
+  static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    __half2 x, y;
+    memcpy(&x, &a, 4);
+    memcpy(&y, &b, 4);
+    x = __hmax2(x, y);
+    memcpy(&a, &x, 4);
+    return a;
+  }
+  static __device__ __forceinline__ float largest(uint32_t word) {
+    return fmaxf(value(word, 0), value(word, 1));
+  }
+};
+
+// Width neighbouring elements in words (a single 16-bit one in the lower half),
+// moved as one access of at most 16 bytes.
+template <typename T, int Width> struct WordVector {
+  static constexpr int kBytes = Width * static_cast<int>(sizeof(T));
+  static constexpr int kWords = kBytes < 4 ? 1 : kBytes / 4;
+  uint32_t at[kWords];
+
+  __device__ __forceinline__ void load(const T *from) {
+    if constexpr (kBytes == 16) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(from);
+      at[0] = v.x;
+      at[1] = v.y;
+      at[2] = v.z;
+      at[3] = v.w;
+    } else if constexpr (kBytes == 8) {
+      const uint2 v = *reinterpret_cast<const uint2 *>(from);
+      at[0] = v.x;
+      at[1] = v.y;
+    } else if constexpr (kBytes == 4) {
+      at[0] = *reinterpret_cast<const uint32_t *>(from);
+    } else {
+      at[0] = *reinterpret_cast<const uint16_t *>(from);
+    }
+  }
+  __device__ __forceinline__ void store(T *to) const {
+    if constexpr (kBytes == 16) {
+      *reinterpret_cast<uint4 *>(to) = make_uint4(at[0], at[1], at[2], at[3]);
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2 *>(to) = make_uint2(at[0], at[1]);
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t *>(to) = at[0];
+    } else {
+      *reinterpret_cast<uint16_t *>(to) = static_cast<uint16_t>(at[0]);
+    }
+  }
 };
 
 // 2^x; 0 for -infinity.

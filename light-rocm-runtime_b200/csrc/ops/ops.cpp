@@ -92,20 +92,23 @@ void check_table(const lro_table_t &table, uint32_t page_size) {
           "the page table holds 2^31 tokens or more");
 }
 
+int32_t stride_of(int64_t elements) {
+  require(elements >= INT32_MIN && elements <= INT32_MAX,
+          "strides must be less than 2^31 elements");
+  return static_cast<int32_t>(elements);
+}
 Cache cache_of(const lro_cache_t &cache) {
-  return {cache.keys,
-          cache.values,
-          cache.key_page_stride,
-          cache.key_token_stride,
-          cache.key_head_stride,
-          cache.value_page_stride,
-          cache.value_token_stride,
-          cache.value_head_stride,
+  return {{cache.keys, stride_of(cache.key_page_stride), stride_of(cache.key_token_stride),
+           stride_of(cache.key_head_stride)},
+          {cache.values, stride_of(cache.value_page_stride), stride_of(cache.value_token_stride),
+           stride_of(cache.value_head_stride)},
           cache.page_count,
           cache.kv_heads,
           Divider::of(cache.page_size)};
 }
-Rows rows_of(const lro_rows_t &rows) { return {rows.data, rows.row_stride, rows.head_stride}; }
+Rows rows_of(const lro_rows_t &rows) {
+  return {rows.data, stride_of(rows.row_stride), stride_of(rows.head_stride)};
+}
 Table table_of(const lro_table_t &table) {
   return {table.pages, table.row_stride, table.rows, table.columns};
 }
@@ -202,6 +205,7 @@ void rope_append(lro_context_t &context, const lro_rope_append_t &a) {
   require(a.heads > 0 && a.heads <= 65536u, "heads out of range");
   require(a.rotary_dim % 2u == 0 && a.rotary_dim <= dim,
           "rotary_dim must be even and at most head_dim");
+  require(a.rotary_dim == 0 || a.table_positions <= 0x7fffffffu, "table_positions out of range");
   require(a.rotary_dim == 0 || (a.cos_table != nullptr && a.sin_table != nullptr &&
                                 multiple_of(a.cos_table, 4) && multiple_of(a.sin_table, 4)),
           "the cos/sin tables are missing");
@@ -231,11 +235,11 @@ void rope_append(lro_context_t &context, const lro_rope_append_t &a) {
       break;
     }
   }
-  const uint32_t per_head = half / width + rest / width;
-  const uint32_t per_value_head = dim / width;
-  const uint64_t turned = (uint64_t{a.heads} + a.cache.kv_heads) * per_head;
-  const uint64_t per_token = turned + uint64_t{a.cache.kv_heads} * per_value_head;
-  require(per_token < (1u << 30), "a token has too many elements");
+  const uint32_t per_head = half / width + rest / width, per_value_head = dim / width;
+  const uint64_t per_token = (uint64_t{a.heads} + a.cache.kv_heads) * per_head;
+  const uint64_t values_per_token = uint64_t{a.cache.kv_heads} * per_value_head;
+  require((per_token + values_per_token) * a.tokens < (uint64_t{1} << 31),
+          "the tokens have too many elements");
   RopeAppendArgs args{};
   args.q = rows_of(a.q);
   args.q_out = rows_of(a.q_out);
@@ -247,19 +251,19 @@ void rope_append(lro_context_t &context, const lro_rope_append_t &a) {
   args.positions = a.positions;
   args.cos_table = a.cos_table;
   args.sin_table = a.sin_table;
-  args.items = per_token * a.tokens;
+  args.items = static_cast<uint32_t>(per_token * a.tokens);
+  args.value_items = static_cast<uint32_t>(values_per_token * a.tokens);
   args.heads = a.heads;
-  args.head_dim = dim;
   args.rotary_dim = a.rotary_dim;
   args.table_positions = a.rotary_dim == 0 ? 0x7fffffffu : a.table_positions;
-  args.items_per_token = static_cast<uint32_t>(per_token);
-  args.turned_items = static_cast<uint32_t>(turned);
-  args.per_token = Divider::of(args.items_per_token);
+  args.per_token = Divider::of(static_cast<uint32_t>(per_token));
   args.per_head = Divider::of(per_head);
-  args.per_value_head = Divider::of(per_value_head);
+  args.values_per_token = Divider::of(static_cast<uint32_t>(values_per_token));
+  args.values_per_head = Divider::of(per_value_head);
   context.launch(std::string("ops_rope_") + (a.interleaved != 0 ? "pairs_" : "half_") +
                      type_name(a.cache.type) + "_x" + std::to_string(width),
-                 ceil_div(args.items, kRopeThreads), kRopeThreads, 0, args);
+                 ceil_div(args.items, kRopeThreads) + ceil_div(args.value_items, kRopeThreads),
+                 kRopeThreads, 0, args);
 }
 
 void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
