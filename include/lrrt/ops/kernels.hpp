@@ -149,10 +149,20 @@ struct PagedAttentionArgs {
   float scale, softcap;
 };
 
-// One run of pages: `rows` rows of page `source` go to page `target`.
+// `rows` rows of page `source` go to page `target`, which may be none (-1).
 struct PageMove {
   int32_t source, target;
-  uint32_t rows, reserved;
+  uint32_t rows;
+  uint32_t row; // of the new table that it is for
+};
+
+// What a row of a forked table takes from its parent, and gets anew.
+struct ForkRow {
+  int32_t parent, last; // -1: none; the parent's last, unfinished page
+  uint32_t length, part; // tokens; those in the last page
+  uint32_t have, need;   // pages that they fill; pages of the new row
+  uint32_t copies;       // 1: the last page has to be copied
+  uint32_t first_new;    // the first of its new pages among the free ones
 };
 
 constexpr uint32_t kPlanBlocks = 8; // one cluster
@@ -166,11 +176,11 @@ struct ForkArgs {
   int64_t table_out_stride;
   int32_t *lengths_out, *status;
   uint32_t rows_out, room, page_count;
+  uint32_t capacity; // tokens of a row of the table
   Divider page;
   uint32_t *owners;    // [page_count]
   int32_t *free_pages; // [page_count]
-  uint32_t *first_new; // [rows_out]
-  uint32_t *first_copy; // [rows_out]
+  ForkRow *rows;       // [rows_out]
   PageMove *moves;     // [rows_out]
   uint32_t *move_count;
 };
@@ -200,8 +210,8 @@ struct MoveArgs {
   const int32_t *sources, *targets;
   uint32_t count; // without move_count
   uint32_t page_count, page_size, segments, row_bytes;
-  uint32_t units_per_move; // layers * 2 * segments * slices
-  Divider per_move, per_segment; // units of a move; slices of a segment
+  Divider per_move;    // units of a move: layers * 2 * segments * slices
+  Divider per_segment; // slices of a segment
   Divider segments_divider;
 };
 

@@ -19,6 +19,12 @@ __device__ __forceinline__ void wait_for_previous_launch() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// The next launch, if it is an overlapped one, may begin and wait for this
+// kernel's end: its blocks are then there at once.
+__device__ __forceinline__ void let_next_launch_begin() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }

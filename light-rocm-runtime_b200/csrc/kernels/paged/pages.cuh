@@ -23,52 +23,61 @@ constexpr uint32_t kPlanAll = kPlanBlocks * kPlanThreads;
 constexpr uint32_t kPlanWarps = kPlanThreads / 32u;
 constexpr uint32_t kNobody = 0xffffffffu; // mark of a page that no row holds
 
-// Exclusive prefix sums over the cluster's threads (rank, then thread) of two
-// counts at once, and their totals. Two cluster barriers.
-struct PlanScan {
-  uint64_t warp_sums[kPlanWarps];
-  uint64_t block_sums[kPlanBlocks];
-};
-
+// Two 32-bit counts in one.
 __device__ __forceinline__ uint64_t pack_counts(uint32_t low, uint32_t high) {
   return uint64_t{high} << 32 | low;
 }
 
-__device__ __forceinline__ uint64_t plan_scan(uint64_t value, PlanScan &scan, uint64_t &total) {
+// Exclusive prefix sums over the cluster's threads (rank, then thread) of two
+// values, and their totals. One cluster barrier; once per kernel.
+struct PlanSums {
+  uint64_t x, y;
+};
+struct PlanScan {
+  PlanSums warps[kPlanWarps];
+  PlanSums blocks[kPlanBlocks];
+};
+
+__device__ __forceinline__ PlanSums plan_scan(PlanSums value, PlanScan &scan, PlanSums &total) {
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5u;
-  uint64_t sum = value;
+  PlanSums sum = value;
 #pragma unroll
   for (uint32_t offset = 1; offset < 32u; offset <<= 1u) {
-    const uint64_t other = __shfl_up_sync(kAllLanes, sum, offset);
+    const uint64_t x = __shfl_up_sync(kAllLanes, sum.x, offset);
+    const uint64_t y = __shfl_up_sync(kAllLanes, sum.y, offset);
     if (lane >= offset) {
-      sum += other;
+      sum.x += x;
+      sum.y += y;
     }
   }
   if (lane == 31u) {
-    scan.warp_sums[warp] = sum;
+    scan.warps[warp] = sum;
   }
   __syncthreads();
-  uint64_t before = 0, block = 0;
-#pragma unroll
+  PlanSums before{sum.x - value.x, sum.y - value.y}, block{0, 0};
+#pragma unroll 4
   for (uint32_t w = 0; w < kPlanWarps; ++w) {
-    const uint64_t s = scan.warp_sums[w];
-    before += w < warp ? s : 0;
-    block += s;
+    const PlanSums s = scan.warps[w];
+    before.x += w < warp ? s.x : 0;
+    before.y += w < warp ? s.y : 0;
+    block.x += s.x;
+    block.y += s.y;
   }
   if (threadIdx.x < kPlanBlocks) {
-    *cluster.map_shared_rank(&scan.block_sums[cluster.block_rank()], threadIdx.x) = block;
+    *cluster.map_shared_rank(&scan.blocks[cluster.block_rank()], threadIdx.x) = block;
   }
   cluster.sync();
-  total = 0;
-#pragma unroll
+  total = {0, 0};
+#pragma unroll 4
   for (uint32_t b = 0; b < kPlanBlocks; ++b) {
-    const uint64_t s = scan.block_sums[b];
-    before += b < cluster.block_rank() ? s : 0;
-    total += s;
+    const PlanSums s = scan.blocks[b];
+    before.x += b < cluster.block_rank() ? s.x : 0;
+    before.y += b < cluster.block_rank() ? s.y : 0;
+    total.x += s.x;
+    total.y += s.y;
   }
-  cluster.sync(); // the sums may be overwritten from here on
-  return before + sum - value;
+  return before;
 }
 
 // The contiguous share of [0, count) of one of the cluster's threads.
@@ -80,40 +89,29 @@ __device__ __forceinline__ void plan_share(uint32_t count, uint32_t &begin, uint
 }
 
 // What a row of the new table takes from its parent.
-struct ForkRow {
-  const int32_t *pages; // the parent's
-  uint32_t length, have, need; // tokens; pages they fill; pages of the new row
-  uint32_t part;               // tokens in the last, unfinished page
-  int32_t last;                // that page, -1: none
-};
-
 __device__ __forceinline__ ForkRow fork_row(const ForkArgs &args, uint32_t row) {
-  ForkRow r{nullptr, 0, 0, 0, 0, -1};
+  ForkRow r{-1, -1, 0, 0, 0, 0, 0, 0};
   const int32_t parent = args.parents[row];
   if (parent < 0 || static_cast<uint32_t>(parent) >= args.table.rows) {
     return r;
   }
-  r.pages = args.table.pages + parent * args.table.row_stride;
-  const uint64_t capacity = uint64_t{args.table.columns} * args.page.divisor;
+  r.parent = parent;
   const int32_t length = args.lengths[parent];
-  r.length = length < 0 ? 0u
-                        : static_cast<uint32_t>(
-                              static_cast<uint64_t>(length) < capacity ? length : capacity);
+  r.length = length < 0 ? 0u : min(static_cast<uint32_t>(length), args.capacity);
   const uint32_t full = args.page.quotient(r.length);
-  r.part = r.length - full * args.page.divisor;
-  r.have = full + (r.part != 0 ? 1u : 0u);
-  const uint64_t wanted =
-      (uint64_t{r.length} + args.room + args.page.divisor - 1u) / args.page.divisor;
-  r.need = wanted < args.table.columns ? static_cast<uint32_t>(wanted) : args.table.columns;
-  if (r.part != 0) {
-    const int32_t page = r.pages[full];
-    r.last = page >= 0 && static_cast<uint32_t>(page) < args.page_count ? page : -1;
+  const uint32_t part = r.length - full * args.page.divisor;
+  r.have = full + (part != 0 ? 1u : 0u);
+  const uint32_t later = r.length + min(args.room, args.capacity - r.length);
+  const uint32_t pages = args.page.quotient(later);
+  r.need = pages + (pages * args.page.divisor != later ? 1u : 0u);
+  if (part != 0) {
+    const int32_t page = args.table.pages[parent * args.table.row_stride + full];
+    if (static_cast<uint32_t>(page) < args.page_count) {
+      r.last = page;
+      r.part = part;
+    }
   }
   return r;
-}
-
-__device__ __forceinline__ bool fork_copies(const ForkArgs &args, const ForkRow &r, uint32_t row) {
-  return r.last >= 0 && __ldcg(args.owners + r.last) != row + 1u;
 }
 
 // owners[page]: kNobody free; 0 held whole by a row (or held outside); s + 1:
@@ -124,154 +122,189 @@ __device__ __forceinline__ void fork_plan(const ForkArgs &args) {
   const uint32_t thread = blockIdx.x * kPlanThreads + threadIdx.x;
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t warp = thread >> 5u;
+  uint32_t row_begin, row_end;
+  plan_share(args.rows_out, row_begin, row_end);
+#pragma unroll 1
+  for (uint32_t row = row_begin; row < row_end; ++row) {
+    const ForkRow r = fork_row(args, row);
+    args.rows[row] = r;
+    args.lengths_out[row] = static_cast<int32_t>(r.length);
+  }
+#pragma unroll 4
   for (uint32_t page = thread; page < args.page_count; page += kPlanAll) {
     args.owners[page] = args.held != nullptr && args.held[page] != 0 ? 0u : kNobody;
   }
   cluster.sync();
+#pragma unroll 1
+  for (uint32_t row = row_begin; row < row_end; ++row) {
+    const int32_t last = args.rows[row].last;
+    if (last >= 0) {
+      atomicMin(args.owners + last, row + 1u);
+    }
+  }
+#pragma unroll 1
   for (uint32_t row = warp; row < args.rows_out; row += kPlanAll / 32u) {
-    const ForkRow r = fork_row(args, row);
+    const ForkRow &r = args.rows[row];
+    const int32_t parent = __ldcg(&r.parent);
+    const uint32_t have = __ldcg(&r.have), length = __ldcg(&r.length);
+    const int32_t *pages = args.table.pages + parent * args.table.row_stride;
     int32_t *out = args.table_out + row * args.table_out_stride;
-    const uint32_t full = r.have - (r.part != 0 ? 1u : 0u);
+    const uint32_t full = args.page.quotient(length);
+#pragma unroll 2
     for (uint32_t column = lane; column < args.table.columns; column += 32u) {
-      const int32_t page = column < r.have ? r.pages[column] : -1;
-      const bool inside = page >= 0 && static_cast<uint32_t>(page) < args.page_count;
+      const int32_t page = column < have ? pages[column] : -1;
+      const bool inside = static_cast<uint32_t>(page) < args.page_count;
       out[column] = inside ? page : -1;
       if (inside && column < full) {
         args.owners[page] = 0; // the lowest there is: no minimum can raise it
       }
     }
-    if (lane == 0) {
-      args.lengths_out[row] = static_cast<int32_t>(r.length);
-      if (r.last >= 0) {
-        atomicMin(args.owners + r.last, row + 1u);
-      }
-    }
   }
   cluster.sync();
-  // Numbers of the free pages below a thread's share, and of the new pages and
-  // copies that the rows before its share want.
-  uint32_t begin, end;
-  plan_share(args.page_count, begin, end);
-  uint32_t free_here = 0;
-  for (uint32_t page = begin; page < end; ++page) {
+  // The free pages below a thread's share; the new pages and the copies that
+  // the rows before its share want.
+  uint32_t page_begin, page_end, free_here = 0, wanted = 0, copies = 0;
+  plan_share(args.page_count, page_begin, page_end);
+#pragma unroll 4
+  for (uint32_t page = page_begin; page < page_end; ++page) {
     free_here += __ldcg(args.owners + page) == kNobody ? 1u : 0u;
   }
-  uint64_t free_total;
-  uint32_t rank = static_cast<uint32_t>(plan_scan(free_here, scan, free_total));
-  for (uint32_t page = begin; page < end; ++page) {
-    if (__ldcg(args.owners + page) == kNobody) {
-      args.free_pages[rank++] = static_cast<int32_t>(page);
-    }
-  }
-  plan_share(args.rows_out, begin, end);
-  uint32_t wanted = 0, copies = 0;
-  for (uint32_t row = begin; row < end; ++row) {
-    const ForkRow r = fork_row(args, row);
-    const uint32_t copy = fork_copies(args, r, row) ? 1u : 0u;
+#pragma unroll 1
+  for (uint32_t row = row_begin; row < row_end; ++row) {
+    const ForkRow r = args.rows[row];
+    const uint32_t copy = r.last >= 0 && __ldcg(args.owners + r.last) != row + 1u ? 1u : 0u;
+    args.rows[row].copies = copy;
     wanted += r.need - r.have + copy;
     copies += copy;
   }
-  uint64_t totals;
-  uint64_t before = plan_scan(pack_counts(wanted, copies), scan, totals);
-  for (uint32_t row = begin; row < end; ++row) {
-    const ForkRow r = fork_row(args, row);
-    const uint32_t copy = fork_copies(args, r, row) ? 1u : 0u;
-    args.first_new[row] = static_cast<uint32_t>(before);
-    args.first_copy[row] = static_cast<uint32_t>(before >> 32);
-    before += pack_counts(r.need - r.have + copy, copy);
-  }
-  cluster.sync();
-  const uint32_t free_pages = static_cast<uint32_t>(free_total);
-  for (uint32_t row = warp; row < args.rows_out; row += kPlanAll / 32u) {
-    const ForkRow r = fork_row(args, row);
-    const bool copy = fork_copies(args, r, row);
-    int32_t *out = args.table_out + row * args.table_out_stride;
-    const uint32_t from = r.have - (copy ? 1u : 0u);
-    const uint32_t first = __ldcg(args.first_new + row);
-    for (uint32_t column = from + lane; column < r.need; column += 32u) {
-      const uint32_t at = first + column - from;
-      const int32_t page = at < free_pages ? __ldcg(args.free_pages + at) : -1;
-      out[column] = page;
-      if (copy && column == from) {
-        args.moves[__ldcg(args.first_copy + row)] = {r.last, page, page >= 0 ? r.part : 0u, 0u};
-      }
+  PlanSums totals;
+  PlanSums before = plan_scan({free_here, pack_counts(wanted, copies)}, scan, totals);
+#pragma unroll 4
+  for (uint32_t page = page_begin; page < page_end; ++page) {
+    if (__ldcg(args.owners + page) == kNobody) {
+      args.free_pages[before.x++] = static_cast<int32_t>(page);
     }
   }
+#pragma unroll 1
+  for (uint32_t row = row_begin; row < row_end; ++row) {
+    const ForkRow r = args.rows[row];
+    args.rows[row].first_new = static_cast<uint32_t>(before.y);
+    if (r.copies != 0) {
+      args.moves[before.y >> 32] = {r.last, -1, r.part, row};
+    }
+    before.y += pack_counts(r.need - r.have + r.copies, r.copies);
+  }
+  cluster.sync();
+  const uint32_t free_pages = static_cast<uint32_t>(totals.x);
+#pragma unroll 1
+  for (uint32_t row = warp; row < args.rows_out; row += kPlanAll / 32u) {
+    const ForkRow &r = args.rows[row];
+    const uint32_t from = __ldcg(&r.have) - __ldcg(&r.copies), need = __ldcg(&r.need);
+    const uint32_t first = __ldcg(&r.first_new);
+    int32_t *out = args.table_out + row * args.table_out_stride;
+#pragma unroll 1
+    for (uint32_t column = from + lane; column < need; column += 32u) {
+      const uint32_t at = first + column - from;
+      out[column] = at < free_pages ? __ldcg(args.free_pages + at) : -1;
+    }
+  }
+  const uint32_t copies_in_all = static_cast<uint32_t>(totals.y >> 32);
+#pragma unroll 1
+  for (uint32_t i = thread; i < copies_in_all; i += kPlanAll) {
+    // A row's copy is the first of its new pages; without one nothing moves.
+    const uint32_t at = __ldcg(&args.rows[__ldcg(&args.moves[i].row)].first_new);
+    args.moves[i].target = at < free_pages ? __ldcg(args.free_pages + at) : -1;
+  }
   if (thread == 0) {
-    const uint32_t all = static_cast<uint32_t>(totals);
+    const uint32_t all = static_cast<uint32_t>(totals.y);
     args.status[0] = static_cast<int32_t>(all > free_pages ? all - free_pages : 0u);
     args.status[1] = static_cast<int32_t>(all < free_pages ? free_pages - all : 0u);
-    *args.move_count = static_cast<uint32_t>(totals >> 32);
+    *args.move_count = copies_in_all;
   }
 }
 
 // marks[page]: kNobody free, 0 held outside, 1 live.
 __device__ __forceinline__ void compact_plan(const CompactArgs &args) {
   __shared__ PlanScan scan;
+  __shared__ uint32_t live_below; // of the live pages, those numbered below `used`
   cg::cluster_group cluster = cg::this_cluster();
   const uint32_t thread = blockIdx.x * kPlanThreads + threadIdx.x;
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t warp = thread >> 5u;
+#pragma unroll 4
   for (uint32_t page = thread; page < args.page_count; page += kPlanAll) {
     args.marks[page] = args.held != nullptr && args.held[page] != 0 ? 0u : kNobody;
   }
   cluster.sync();
+#pragma unroll 1
   for (uint32_t row = warp; row < args.table.rows; row += kPlanAll / 32u) {
     const int32_t *pages = args.table.pages + row * args.table.row_stride;
+#pragma unroll 2
     for (uint32_t column = lane; column < args.table.columns; column += 32u) {
       const int32_t page = pages[column];
-      if (page >= 0 && static_cast<uint32_t>(page) < args.page_count &&
+      if (static_cast<uint32_t>(page) < args.page_count &&
           (args.held == nullptr || args.held[page] == 0)) {
         args.marks[page] = 1u;
       }
     }
   }
   cluster.sync();
-  uint32_t begin, end;
+  uint32_t begin, end, used_here = 0, live_here = 0;
   plan_share(args.page_count, begin, end);
-  uint32_t used_here = 0;
-  for (uint32_t page = begin; page < end; ++page) {
-    used_here += __ldcg(args.marks + page) != kNobody ? 1u : 0u;
-  }
-  uint64_t total;
-  plan_scan(used_here, scan, total);
-  const uint32_t used = static_cast<uint32_t>(total);
-  uint32_t high_here = 0, low_here = 0;
+#pragma unroll 4
   for (uint32_t page = begin; page < end; ++page) {
     const uint32_t mark = __ldcg(args.marks + page);
-    high_here += mark == 1u && page >= used ? 1u : 0u;
-    low_here += mark == kNobody && page < used ? 1u : 0u;
+    used_here += mark != kNobody ? 1u : 0u;
+    live_here += mark == 1u ? 1u : 0u;
   }
-  uint64_t totals;
-  const uint64_t before = plan_scan(pack_counts(high_here, low_here), scan, totals);
-  uint32_t high = static_cast<uint32_t>(before), low = static_cast<uint32_t>(before >> 32);
+  PlanSums totals;
+  PlanSums before = plan_scan({used_here, live_here}, scan, totals);
+  const uint32_t used = static_cast<uint32_t>(totals.x), live = static_cast<uint32_t>(totals.y);
+  // The live pages before each live page, and the free pages in their order: of
+  // the pages below a free one all that are not used are free.
+#pragma unroll 1
   for (uint32_t page = begin; page < end; ++page) {
     const uint32_t mark = __ldcg(args.marks + page);
-    if (mark == kNobody && page < used) {
-      args.free_pages[low++] = static_cast<int32_t>(page);
+    if (page == used) {
+      for (uint32_t b = 0; b < kPlanBlocks; ++b) {
+        *cluster.map_shared_rank(&live_below, b) = static_cast<uint32_t>(before.y);
+      }
     }
-    if (mark == 1u && page >= used) {
-      args.ranks[page] = high;
-      args.moves[high++].source = static_cast<int32_t>(page);
+    if (mark == kNobody) {
+      args.free_pages[page - before.x] = static_cast<int32_t>(page);
+    } else {
+      args.ranks[page] = static_cast<uint32_t>(before.y);
+      ++before.x;
+      before.y += mark == 1u ? 1u : 0u;
     }
+  }
+  if (used == args.page_count && threadIdx.x == 0) {
+    live_below = live; // no page lies above
   }
   cluster.sync();
   // As many free pages lie below `used` as used ones lie above, so every
   // moved page has a place.
-  const uint32_t moved = static_cast<uint32_t>(totals);
-  for (uint32_t i = thread; i < moved; i += kPlanAll) {
-    args.moves[i].target = __ldcg(args.free_pages + i);
-    args.moves[i].rows = args.page_size;
+  const uint32_t below = live_below, moved = live - below;
+  begin = max(begin, used);
+#pragma unroll 1
+  for (uint32_t page = begin; page < end; ++page) {
+    if (__ldcg(args.marks + page) == 1u) {
+      const uint32_t rank = args.ranks[page] - below;
+      args.moves[rank] = {static_cast<int32_t>(page), __ldcg(args.free_pages + rank),
+                          args.page_size, 0u};
+    }
   }
+#pragma unroll 1
   for (uint32_t row = warp; row < args.table.rows; row += kPlanAll / 32u) {
     const int32_t *pages = args.table.pages + row * args.table.row_stride;
     int32_t *out = args.table_out + row * args.table_out_stride;
+#pragma unroll 2
     for (uint32_t column = lane; column < args.table.columns; column += 32u) {
       int32_t page = pages[column];
-      if (page < 0 || static_cast<uint32_t>(page) >= args.page_count) {
+      if (static_cast<uint32_t>(page) >= args.page_count) {
         page = -1;
       } else if (static_cast<uint32_t>(page) >= used && __ldcg(args.marks + page) == 1u) {
-        page = __ldcg(args.free_pages + __ldcg(args.ranks + page));
+        page = __ldcg(args.free_pages + __ldcg(args.ranks + page) - below);
       }
       out[column] = page;
     }
@@ -287,15 +320,18 @@ __device__ __forceinline__ void compact_plan(const CompactArgs &args) {
 // is kMoveSliceVectors vectors, eight loads in flight per lane.
 template <typename V> __device__ __forceinline__ void move_pages(const MoveArgs &args) {
   const uint32_t moves = args.move_count != nullptr ? __ldcg(args.move_count) : args.count;
-  const uint64_t units = uint64_t{moves} * args.units_per_move;
   const uint32_t lane = threadIdx.x & 31u;
-  const uint64_t warps = uint64_t{gridDim.x} * (kMoveThreads / 32u);
-  for (uint64_t unit = (uint64_t{blockIdx.x} * kMoveThreads + threadIdx.x) / 32u; unit < units;
-       unit += warps) {
-    const uint32_t index = unit < (uint64_t{1} << 31)
-                               ? args.per_move.quotient(static_cast<uint32_t>(unit))
-                               : static_cast<uint32_t>(unit / args.units_per_move);
-    const uint32_t in_move = static_cast<uint32_t>(unit - uint64_t{index} * args.units_per_move);
+  const uint32_t warp = (blockIdx.x * kMoveThreads + threadIdx.x) / 32u;
+  const uint32_t warps = gridDim.x * (kMoveThreads / 32u);
+  const uint32_t units = args.per_move.divisor;
+  // The grid's warps are so many moves and units ahead of one another.
+  const uint32_t moves_ahead = args.per_move.quotient(warps);
+  const uint32_t units_ahead = warps - moves_ahead * units;
+  uint32_t index = args.per_move.quotient(warp), in_move = warp - index * units;
+#pragma unroll 1
+  for (; index < moves;
+       index += moves_ahead, in_move += units_ahead, index += in_move >= units ? 1u : 0u,
+       in_move -= in_move >= units ? units : 0u) {
     const uint32_t segment_index = args.per_segment.quotient(in_move);
     const uint32_t slice = in_move - segment_index * args.per_segment.divisor;
     const uint32_t plane = args.segments_divider.quotient(segment_index);

@@ -54,12 +54,14 @@ LRRT_ATTENTION(f16_256x8, __half, 256, 1)
 extern "C" __global__ void __cluster_dims__(kPlanBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     ops_fork_plan(const __grid_constant__ ForkArgs args) {
   wait_for_previous_launch();
+  let_next_launch_begin();
   fork_plan(args);
 }
 
 extern "C" __global__ void __cluster_dims__(kPlanBlocks, 1, 1) __launch_bounds__(kPlanThreads)
     ops_compact_plan(const __grid_constant__ CompactArgs args) {
   wait_for_previous_launch();
+  let_next_launch_begin();
   compact_plan(args);
 }
 

@@ -360,8 +360,7 @@ bool pool_moves(const lro_pool_t &pool, MoveArgs &args) {
   args.page_size = pool.page_size;
   args.segments = pool.segments;
   args.row_bytes = pool.row_bytes;
-  args.units_per_move = static_cast<uint32_t>(units);
-  args.per_move = Divider::of(args.units_per_move);
+  args.per_move = Divider::of(static_cast<uint32_t>(units));
   args.per_segment = Divider::of(static_cast<uint32_t>(slices));
   args.segments_divider = Divider::of(pool.segments);
   return wide;
@@ -369,7 +368,7 @@ bool pool_moves(const lro_pool_t &pool, MoveArgs &args) {
 
 // At most `most` moves, one warp per unit, at most eight blocks per SM.
 void launch_moves(lro_context_t &context, const MoveArgs &args, bool wide, uint64_t most) {
-  const uint64_t blocks = ceil_div(most * args.units_per_move, kMoveThreads / 32u);
+  const uint64_t blocks = ceil_div(most * args.per_move.divisor, kMoveThreads / 32u);
   context.launch(wide ? "ops_move_pages_16" : "ops_move_pages_4",
                  std::min<uint64_t>(blocks, uint64_t{context.sms} * 8u), kMoveThreads, 0, args);
 }
@@ -389,12 +388,10 @@ void pages_fork(lro_context_t &context, const lro_pages_fork_t &a) {
   require(a.rows_out == 0 || a.table.columns == 0 || a.table_out != a.table.pages,
           "table_out must not be the table");
   const size_t rows = a.rows_out, pages = a.pool.page_count;
-  size_t bytes = 256;
-  const size_t moves_at = bytes, owners_at = moves_at + aligned(sizeof(PageMove) * rows),
-               free_at = owners_at + aligned(4u * pages), new_at = free_at + aligned(4u * pages),
-               copy_at = new_at + aligned(4u * rows);
-  bytes = copy_at + aligned(4u * rows);
-  context.reserve(bytes);
+  const size_t moves_at = 256, rows_at = moves_at + aligned(sizeof(PageMove) * rows),
+               owners_at = rows_at + aligned(sizeof(ForkRow) * rows),
+               free_at = owners_at + aligned(4u * pages);
+  context.reserve(free_at + aligned(4u * pages));
   auto *scratch = static_cast<unsigned char *>(context.scratch->data());
   ForkArgs args{};
   args.table = table_of(a.table);
@@ -407,14 +404,14 @@ void pages_fork(lro_context_t &context, const lro_pages_fork_t &a) {
   args.status = a.status;
   args.rows_out = a.rows_out;
   args.room = a.room;
+  args.capacity = a.table.columns * a.pool.page_size;
   args.page_count = a.pool.page_count;
   args.page = Divider::of(a.pool.page_size);
   args.move_count = reinterpret_cast<uint32_t *>(scratch);
   args.moves = reinterpret_cast<PageMove *>(scratch + moves_at);
   args.owners = reinterpret_cast<uint32_t *>(scratch + owners_at);
   args.free_pages = reinterpret_cast<int32_t *>(scratch + free_at);
-  args.first_new = reinterpret_cast<uint32_t *>(scratch + new_at);
-  args.first_copy = reinterpret_cast<uint32_t *>(scratch + copy_at);
+  args.rows = reinterpret_cast<ForkRow *>(scratch + rows_at);
   context.launch("ops_fork_plan", kPlanBlocks, kPlanThreads, 0, args);
   if (a.rows_out != 0 && a.pool.page_size > 1) { // pages of one token are never unfinished
     moves.moves = args.moves;
