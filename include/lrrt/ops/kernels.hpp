@@ -167,6 +167,19 @@ struct ForkRow {
 
 constexpr uint32_t kPlanBlocks = 8; // one cluster
 constexpr uint32_t kPlanThreads = 512;
+constexpr uint32_t kPlanThreadsAlone = 1024; // of a block that plans by itself
+constexpr uint32_t kPlanAloneBytes = 200u * 1024u; // of working arrays, in shared memory
+constexpr uint32_t kPlanAloneEntries = 32768;      // of the table
+
+// Working arrays of a plan: [row_count] rows (fork), and [page_count] marks,
+// free pages and ranks (compact).
+struct PlanArrays {
+  ForkRow *rows;
+  uint32_t *marks;
+  int32_t *free_pages;
+  uint32_t *ranks;
+  uint32_t row_count;
+};
 
 struct ForkArgs {
   Table table;
@@ -178,10 +191,8 @@ struct ForkArgs {
   uint32_t rows_out, room, page_count;
   uint32_t capacity; // tokens of a row of the table
   Divider page;
-  uint32_t *owners;    // [page_count]
-  int32_t *free_pages; // [page_count]
-  ForkRow *rows;       // [rows_out]
-  PageMove *moves;     // [rows_out]
+  PlanArrays arrays;
+  PageMove *moves; // [rows_out]
   uint32_t *move_count;
 };
 
@@ -192,10 +203,8 @@ struct CompactArgs {
   int64_t table_out_stride;
   int32_t *status;
   uint32_t page_count, page_size;
-  uint32_t *marks;     // [page_count]
-  int32_t *free_pages; // [page_count]
-  uint32_t *ranks;     // [page_count]
-  PageMove *moves;     // [page_count]
+  PlanArrays arrays;
+  PageMove *moves; // [page_count]
   uint32_t *move_count;
 };
 

@@ -1,13 +1,14 @@
 // Sharing, splitting, freeing and compacting the pages of a cache.
 //
-// A plan kernel (one cluster of eight blocks) works out the new tables and a
-// list of page moves; a copy kernel over the whole GPU then moves the rows of
+// A plan kernel works out the new tables and a list of page moves: one block
+// with its working arrays in shared memory where they fit, else a cluster of
+// eight with them in the workspace. A copy kernel over the whole GPU then moves the rows of
 // every layer. Which pages are free follows from the tables alone, so no
 // reference counts are kept that could drift from them. Every choice is the
 // lowest number, so the results do not depend on the order of threads.
 //
-// The plan is bound by latency (a few dependent reads of small tables, joined
-// by cluster barriers), the copy by memory bandwidth.
+// The plan is bound by latency (a few dependent reads of small tables between
+// barriers), the copy by memory bandwidth.
 #ifndef LRRT_PAGED_PAGES_CUH_
 #define LRRT_PAGED_PAGES_CUH_
 
@@ -19,27 +20,68 @@ namespace lrrt::ops {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t kPlanAll = kPlanBlocks * kPlanThreads;
-constexpr uint32_t kPlanWarps = kPlanThreads / 32u;
 constexpr uint32_t kNobody = 0xffffffffu; // mark of a page that no row holds
+
+// A block alone, or the cluster: its threads, its barrier, and reads of what
+// other threads of it wrote (past the L1 cache where they are of other SMs).
+template <bool Clustered> struct Plan {
+  static constexpr uint32_t kBlocks = Clustered ? kPlanBlocks : 1u;
+  static constexpr uint32_t kThreads = Clustered ? kPlanThreads : kPlanThreadsAlone;
+  static constexpr uint32_t kAll = kBlocks * kThreads;
+  static constexpr uint32_t kWarps = kThreads / 32u;
+
+  static __device__ __forceinline__ uint32_t rank() {
+    return Clustered ? cg::this_cluster().block_rank() : 0u;
+  }
+  static __device__ __forceinline__ void sync() {
+    if constexpr (Clustered) {
+      cg::this_cluster().sync();
+    } else {
+      __syncthreads();
+    }
+  }
+  template <typename T> static __device__ __forceinline__ T read(const T *from) {
+    if constexpr (Clustered) {
+      return __ldcg(from);
+    } else {
+      return *from;
+    }
+  }
+  // Shared variables of every block of it.
+  template <typename T> static __device__ __forceinline__ T *of_block(T *mine, uint32_t block) {
+    if constexpr (Clustered) {
+      return cg::this_cluster().map_shared_rank(mine, block);
+    } else {
+      return mine;
+    }
+  }
+  // The contiguous share of [0, count) of one of its threads.
+  static __device__ __forceinline__ void share(uint32_t count, uint32_t &begin, uint32_t &end) {
+    const uint32_t each = (count + kAll - 1u) / kAll;
+    const uint64_t first = uint64_t{blockIdx.x * kThreads + threadIdx.x} * each;
+    begin = first < count ? static_cast<uint32_t>(first) : count;
+    end = count - begin < each ? count : begin + each;
+  }
+};
 
 // Two 32-bit counts in one.
 __device__ __forceinline__ uint64_t pack_counts(uint32_t low, uint32_t high) {
   return uint64_t{high} << 32 | low;
 }
 
-// Exclusive prefix sums over the cluster's threads (rank, then thread) of two
-// values, and their totals. One cluster barrier; once per kernel.
+// Exclusive prefix sums over the threads (rank, then thread) of two values, and
+// their totals. Once per kernel.
 struct PlanSums {
   uint64_t x, y;
 };
-struct PlanScan {
-  PlanSums warps[kPlanWarps];
-  PlanSums blocks[kPlanBlocks];
+template <typename P> struct PlanScan {
+  PlanSums warps[P::kWarps];
+  PlanSums blocks[P::kBlocks];
 };
 
-__device__ __forceinline__ PlanSums plan_scan(PlanSums value, PlanScan &scan, PlanSums &total) {
-  cg::cluster_group cluster = cg::this_cluster();
+template <typename P>
+__device__ __forceinline__ PlanSums plan_scan(PlanSums value, PlanScan<P> &scan,
+                                              PlanSums &total) {
   const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5u;
   PlanSums sum = value;
 #pragma unroll
@@ -57,35 +99,41 @@ __device__ __forceinline__ PlanSums plan_scan(PlanSums value, PlanScan &scan, Pl
   __syncthreads();
   PlanSums before{sum.x - value.x, sum.y - value.y}, block{0, 0};
 #pragma unroll 4
-  for (uint32_t w = 0; w < kPlanWarps; ++w) {
+  for (uint32_t w = 0; w < P::kWarps; ++w) {
     const PlanSums s = scan.warps[w];
     before.x += w < warp ? s.x : 0;
     before.y += w < warp ? s.y : 0;
     block.x += s.x;
     block.y += s.y;
   }
-  if (threadIdx.x < kPlanBlocks) {
-    *cluster.map_shared_rank(&scan.blocks[cluster.block_rank()], threadIdx.x) = block;
+  if (threadIdx.x < P::kBlocks) {
+    *P::of_block(&scan.blocks[P::rank()], threadIdx.x) = block;
   }
-  cluster.sync();
+  P::sync();
   total = {0, 0};
 #pragma unroll 4
-  for (uint32_t b = 0; b < kPlanBlocks; ++b) {
+  for (uint32_t b = 0; b < P::kBlocks; ++b) {
     const PlanSums s = scan.blocks[b];
-    before.x += b < cluster.block_rank() ? s.x : 0;
-    before.y += b < cluster.block_rank() ? s.y : 0;
+    before.x += b < P::rank() ? s.x : 0;
+    before.y += b < P::rank() ? s.y : 0;
     total.x += s.x;
     total.y += s.y;
   }
   return before;
 }
 
-// The contiguous share of [0, count) of one of the cluster's threads.
-__device__ __forceinline__ void plan_share(uint32_t count, uint32_t &begin, uint32_t &end) {
-  const uint32_t share = (count + kPlanAll - 1u) / kPlanAll;
-  const uint64_t first = uint64_t{blockIdx.x * kPlanThreads + threadIdx.x} * share;
-  begin = first < count ? static_cast<uint32_t>(first) : count;
-  end = count - begin < share ? count : begin + share;
+// The working arrays: in shared memory for a block alone.
+template <typename P>
+__device__ __forceinline__ PlanArrays plan_arrays(const PlanArrays &arrays, uint32_t pages) {
+  if constexpr (P::kBlocks != 1u) {
+    return arrays;
+  } else {
+    extern __shared__ __align__(16) unsigned char plan_memory[];
+    auto *rows = reinterpret_cast<ForkRow *>(plan_memory);
+    auto *marks = reinterpret_cast<uint32_t *>(rows + arrays.row_count);
+    return {rows, marks, reinterpret_cast<int32_t *>(marks + pages), marks + 2u * size_t{pages},
+            arrays.row_count};
+  }
 }
 
 // What a row of the new table takes from its parent.
@@ -116,37 +164,38 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs &args, uint32_t row) 
 
 // owners[page]: kNobody free; 0 held whole by a row (or held outside); s + 1:
 // the unfinished last page of row s, the lowest that has it.
-__device__ __forceinline__ void fork_plan(const ForkArgs &args) {
-  __shared__ PlanScan scan;
-  cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t thread = blockIdx.x * kPlanThreads + threadIdx.x;
+template <typename P> __device__ __forceinline__ void fork_plan(const ForkArgs &args) {
+  __shared__ PlanScan<P> scan;
+  const PlanArrays arrays = plan_arrays<P>(args.arrays, args.page_count);
+  uint32_t *owners = arrays.marks;
+  const uint32_t thread = blockIdx.x * P::kThreads + threadIdx.x;
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t warp = thread >> 5u;
   uint32_t row_begin, row_end;
-  plan_share(args.rows_out, row_begin, row_end);
+  P::share(args.rows_out, row_begin, row_end);
 #pragma unroll 1
   for (uint32_t row = row_begin; row < row_end; ++row) {
     const ForkRow r = fork_row(args, row);
-    args.rows[row] = r;
+    arrays.rows[row] = r;
     args.lengths_out[row] = static_cast<int32_t>(r.length);
   }
 #pragma unroll 4
-  for (uint32_t page = thread; page < args.page_count; page += kPlanAll) {
-    args.owners[page] = args.held != nullptr && args.held[page] != 0 ? 0u : kNobody;
+  for (uint32_t page = thread; page < args.page_count; page += P::kAll) {
+    owners[page] = args.held != nullptr && args.held[page] != 0 ? 0u : kNobody;
   }
-  cluster.sync();
+  P::sync();
 #pragma unroll 1
   for (uint32_t row = row_begin; row < row_end; ++row) {
-    const int32_t last = args.rows[row].last;
+    const int32_t last = arrays.rows[row].last;
     if (last >= 0) {
-      atomicMin(args.owners + last, row + 1u);
+      atomicMin(owners + last, row + 1u);
     }
   }
 #pragma unroll 1
-  for (uint32_t row = warp; row < args.rows_out; row += kPlanAll / 32u) {
-    const ForkRow &r = args.rows[row];
-    const int32_t parent = __ldcg(&r.parent);
-    const uint32_t have = __ldcg(&r.have), length = __ldcg(&r.length);
+  for (uint32_t row = warp; row < args.rows_out; row += P::kAll / 32u) {
+    const ForkRow &r = arrays.rows[row];
+    const int32_t parent = P::read(&r.parent);
+    const uint32_t have = P::read(&r.have), length = P::read(&r.length);
     const int32_t *pages = args.table.pages + parent * args.table.row_stride;
     int32_t *out = args.table_out + row * args.table_out_stride;
     const uint32_t full = args.page.quotient(length);
@@ -156,24 +205,24 @@ __device__ __forceinline__ void fork_plan(const ForkArgs &args) {
       const bool inside = static_cast<uint32_t>(page) < args.page_count;
       out[column] = inside ? page : -1;
       if (inside && column < full) {
-        args.owners[page] = 0; // the lowest there is: no minimum can raise it
+        owners[page] = 0; // the lowest there is: no minimum can raise it
       }
     }
   }
-  cluster.sync();
+  P::sync();
   // The free pages below a thread's share; the new pages and the copies that
   // the rows before its share want.
   uint32_t page_begin, page_end, free_here = 0, wanted = 0, copies = 0;
-  plan_share(args.page_count, page_begin, page_end);
+  P::share(args.page_count, page_begin, page_end);
 #pragma unroll 4
   for (uint32_t page = page_begin; page < page_end; ++page) {
-    free_here += __ldcg(args.owners + page) == kNobody ? 1u : 0u;
+    free_here += P::read(owners + page) == kNobody ? 1u : 0u;
   }
 #pragma unroll 1
   for (uint32_t row = row_begin; row < row_end; ++row) {
-    const ForkRow r = args.rows[row];
-    const uint32_t copy = r.last >= 0 && __ldcg(args.owners + r.last) != row + 1u ? 1u : 0u;
-    args.rows[row].copies = copy;
+    const ForkRow r = arrays.rows[row];
+    const uint32_t copy = r.last >= 0 && P::read(owners + r.last) != row + 1u ? 1u : 0u;
+    arrays.rows[row].copies = copy;
     wanted += r.need - r.have + copy;
     copies += copy;
   }
@@ -181,39 +230,39 @@ __device__ __forceinline__ void fork_plan(const ForkArgs &args) {
   PlanSums before = plan_scan({free_here, pack_counts(wanted, copies)}, scan, totals);
 #pragma unroll 4
   for (uint32_t page = page_begin; page < page_end; ++page) {
-    if (__ldcg(args.owners + page) == kNobody) {
-      args.free_pages[before.x++] = static_cast<int32_t>(page);
+    if (P::read(owners + page) == kNobody) {
+      arrays.free_pages[before.x++] = static_cast<int32_t>(page);
     }
   }
 #pragma unroll 1
   for (uint32_t row = row_begin; row < row_end; ++row) {
-    const ForkRow r = args.rows[row];
-    args.rows[row].first_new = static_cast<uint32_t>(before.y);
+    const ForkRow r = arrays.rows[row];
+    arrays.rows[row].first_new = static_cast<uint32_t>(before.y);
     if (r.copies != 0) {
       args.moves[before.y >> 32] = {r.last, -1, r.part, row};
     }
     before.y += pack_counts(r.need - r.have + r.copies, r.copies);
   }
-  cluster.sync();
+  P::sync();
   const uint32_t free_pages = static_cast<uint32_t>(totals.x);
 #pragma unroll 1
-  for (uint32_t row = warp; row < args.rows_out; row += kPlanAll / 32u) {
-    const ForkRow &r = args.rows[row];
-    const uint32_t from = __ldcg(&r.have) - __ldcg(&r.copies), need = __ldcg(&r.need);
-    const uint32_t first = __ldcg(&r.first_new);
+  for (uint32_t row = warp; row < args.rows_out; row += P::kAll / 32u) {
+    const ForkRow &r = arrays.rows[row];
+    const uint32_t from = P::read(&r.have) - P::read(&r.copies), need = P::read(&r.need);
+    const uint32_t first = P::read(&r.first_new);
     int32_t *out = args.table_out + row * args.table_out_stride;
 #pragma unroll 1
     for (uint32_t column = from + lane; column < need; column += 32u) {
       const uint32_t at = first + column - from;
-      out[column] = at < free_pages ? __ldcg(args.free_pages + at) : -1;
+      out[column] = at < free_pages ? P::read(arrays.free_pages + at) : -1;
     }
   }
   const uint32_t copies_in_all = static_cast<uint32_t>(totals.y >> 32);
 #pragma unroll 1
-  for (uint32_t i = thread; i < copies_in_all; i += kPlanAll) {
+  for (uint32_t i = thread; i < copies_in_all; i += P::kAll) {
     // A row's copy is the first of its new pages; without one nothing moves.
-    const uint32_t at = __ldcg(&args.rows[__ldcg(&args.moves[i].row)].first_new);
-    args.moves[i].target = at < free_pages ? __ldcg(args.free_pages + at) : -1;
+    const uint32_t at = P::read(&arrays.rows[P::read(&args.moves[i].row)].first_new);
+    args.moves[i].target = at < free_pages ? P::read(arrays.free_pages + at) : -1;
   }
   if (thread == 0) {
     const uint32_t all = static_cast<uint32_t>(totals.y);
@@ -224,36 +273,36 @@ __device__ __forceinline__ void fork_plan(const ForkArgs &args) {
 }
 
 // marks[page]: kNobody free, 0 held outside, 1 live.
-__device__ __forceinline__ void compact_plan(const CompactArgs &args) {
-  __shared__ PlanScan scan;
+template <typename P> __device__ __forceinline__ void compact_plan(const CompactArgs &args) {
+  __shared__ PlanScan<P> scan;
+  const PlanArrays arrays = plan_arrays<P>(args.arrays, args.page_count);
   __shared__ uint32_t live_below; // of the live pages, those numbered below `used`
-  cg::cluster_group cluster = cg::this_cluster();
-  const uint32_t thread = blockIdx.x * kPlanThreads + threadIdx.x;
+  const uint32_t thread = blockIdx.x * P::kThreads + threadIdx.x;
   const uint32_t lane = threadIdx.x & 31u;
   const uint32_t warp = thread >> 5u;
 #pragma unroll 4
-  for (uint32_t page = thread; page < args.page_count; page += kPlanAll) {
-    args.marks[page] = args.held != nullptr && args.held[page] != 0 ? 0u : kNobody;
+  for (uint32_t page = thread; page < args.page_count; page += P::kAll) {
+    arrays.marks[page] = args.held != nullptr && args.held[page] != 0 ? 0u : kNobody;
   }
-  cluster.sync();
+  P::sync();
 #pragma unroll 1
-  for (uint32_t row = warp; row < args.table.rows; row += kPlanAll / 32u) {
+  for (uint32_t row = warp; row < args.table.rows; row += P::kAll / 32u) {
     const int32_t *pages = args.table.pages + row * args.table.row_stride;
 #pragma unroll 2
     for (uint32_t column = lane; column < args.table.columns; column += 32u) {
       const int32_t page = pages[column];
       if (static_cast<uint32_t>(page) < args.page_count &&
           (args.held == nullptr || args.held[page] == 0)) {
-        args.marks[page] = 1u;
+        arrays.marks[page] = 1u;
       }
     }
   }
-  cluster.sync();
+  P::sync();
   uint32_t begin, end, used_here = 0, live_here = 0;
-  plan_share(args.page_count, begin, end);
+  P::share(args.page_count, begin, end);
 #pragma unroll 4
   for (uint32_t page = begin; page < end; ++page) {
-    const uint32_t mark = __ldcg(args.marks + page);
+    const uint32_t mark = P::read(arrays.marks + page);
     used_here += mark != kNobody ? 1u : 0u;
     live_here += mark == 1u ? 1u : 0u;
   }
@@ -264,16 +313,16 @@ __device__ __forceinline__ void compact_plan(const CompactArgs &args) {
   // the pages below a free one all that are not used are free.
 #pragma unroll 1
   for (uint32_t page = begin; page < end; ++page) {
-    const uint32_t mark = __ldcg(args.marks + page);
+    const uint32_t mark = P::read(arrays.marks + page);
     if (page == used) {
-      for (uint32_t b = 0; b < kPlanBlocks; ++b) {
-        *cluster.map_shared_rank(&live_below, b) = static_cast<uint32_t>(before.y);
+      for (uint32_t b = 0; b < P::kBlocks; ++b) {
+        *P::of_block(&live_below, b) = static_cast<uint32_t>(before.y);
       }
     }
     if (mark == kNobody) {
-      args.free_pages[page - before.x] = static_cast<int32_t>(page);
+      arrays.free_pages[page - before.x] = static_cast<int32_t>(page);
     } else {
-      args.ranks[page] = static_cast<uint32_t>(before.y);
+      arrays.ranks[page] = static_cast<uint32_t>(before.y);
       ++before.x;
       before.y += mark == 1u ? 1u : 0u;
     }
@@ -281,21 +330,21 @@ __device__ __forceinline__ void compact_plan(const CompactArgs &args) {
   if (used == args.page_count && threadIdx.x == 0) {
     live_below = live; // no page lies above
   }
-  cluster.sync();
+  P::sync();
   // As many free pages lie below `used` as used ones lie above, so every
   // moved page has a place.
   const uint32_t below = live_below, moved = live - below;
   begin = max(begin, used);
 #pragma unroll 1
   for (uint32_t page = begin; page < end; ++page) {
-    if (__ldcg(args.marks + page) == 1u) {
-      const uint32_t rank = args.ranks[page] - below;
-      args.moves[rank] = {static_cast<int32_t>(page), __ldcg(args.free_pages + rank),
+    if (P::read(arrays.marks + page) == 1u) {
+      const uint32_t rank = arrays.ranks[page] - below;
+      args.moves[rank] = {static_cast<int32_t>(page), P::read(arrays.free_pages + rank),
                           args.page_size, 0u};
     }
   }
 #pragma unroll 1
-  for (uint32_t row = warp; row < args.table.rows; row += kPlanAll / 32u) {
+  for (uint32_t row = warp; row < args.table.rows; row += P::kAll / 32u) {
     const int32_t *pages = args.table.pages + row * args.table.row_stride;
     int32_t *out = args.table_out + row * args.table_out_stride;
 #pragma unroll 2
@@ -303,8 +352,8 @@ __device__ __forceinline__ void compact_plan(const CompactArgs &args) {
       int32_t page = pages[column];
       if (static_cast<uint32_t>(page) >= args.page_count) {
         page = -1;
-      } else if (static_cast<uint32_t>(page) >= used && __ldcg(args.marks + page) == 1u) {
-        page = __ldcg(args.free_pages + __ldcg(args.ranks + page) - below);
+      } else if (static_cast<uint32_t>(page) >= used && P::read(arrays.marks + page) == 1u) {
+        page = P::read(arrays.free_pages + P::read(arrays.ranks + page) - below);
       }
       out[column] = page;
     }

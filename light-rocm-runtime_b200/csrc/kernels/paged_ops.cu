@@ -51,19 +51,22 @@ LRRT_ATTENTION(f16_128x8, __half, 128, 1)
 LRRT_ATTENTION(f16_128x16, __half, 128, 2)
 LRRT_ATTENTION(f16_256x8, __half, 256, 1)
 
-extern "C" __global__ void __cluster_dims__(kPlanBlocks, 1, 1) __launch_bounds__(kPlanThreads)
-    ops_fork_plan(const __grid_constant__ ForkArgs args) {
-  wait_for_previous_launch();
-  let_next_launch_begin();
-  fork_plan(args);
-}
+#define LRRT_PLAN(name, args_type)                                                                \
+  extern "C" __global__ void __cluster_dims__(kPlanBlocks, 1, 1) __launch_bounds__(kPlanThreads)  \
+      ops_##name(const __grid_constant__ args_type args) {                                        \
+    wait_for_previous_launch();                                                                   \
+    let_next_launch_begin();                                                                      \
+    name<Plan<true>>(args);                                                                       \
+  }                                                                                               \
+  extern "C" __global__ void __launch_bounds__(kPlanThreadsAlone)                                 \
+      ops_##name##_alone(const __grid_constant__ args_type args) {                                \
+    wait_for_previous_launch();                                                                   \
+    let_next_launch_begin();                                                                      \
+    name<Plan<false>>(args);                                                                      \
+  }
 
-extern "C" __global__ void __cluster_dims__(kPlanBlocks, 1, 1) __launch_bounds__(kPlanThreads)
-    ops_compact_plan(const __grid_constant__ CompactArgs args) {
-  wait_for_previous_launch();
-  let_next_launch_begin();
-  compact_plan(args);
-}
+LRRT_PLAN(fork_plan, ForkArgs)
+LRRT_PLAN(compact_plan, CompactArgs)
 
 #define LRRT_MOVE(bytes, type)                                                                    \
   extern "C" __global__ void __launch_bounds__(kMoveThreads)                                      \

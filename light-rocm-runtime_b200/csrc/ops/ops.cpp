@@ -373,6 +373,35 @@ void launch_moves(lro_context_t &context, const MoveArgs &args, bool wide, uint6
                  std::min<uint64_t>(blocks, uint64_t{context.sms} * 8u), kMoveThreads, 0, args);
 }
 
+// Workspace of a plan: the number of moves, the moves, and the arrays.
+void plan_memory(lro_context_t &context, size_t rows, size_t pages, size_t moves,
+                 PlanArrays &arrays, PageMove *&list, uint32_t *&list_count) {
+  const size_t rows_at = 256u + aligned(sizeof(PageMove) * moves),
+               marks_at = rows_at + aligned(sizeof(ForkRow) * rows),
+               free_at = marks_at + aligned(4u * pages), ranks_at = free_at + aligned(4u * pages);
+  context.reserve(ranks_at + aligned(4u * pages));
+  auto *scratch = static_cast<unsigned char *>(context.scratch->data());
+  list_count = reinterpret_cast<uint32_t *>(scratch);
+  list = reinterpret_cast<PageMove *>(scratch + 256);
+  arrays = {reinterpret_cast<ForkRow *>(scratch + rows_at),
+            reinterpret_cast<uint32_t *>(scratch + marks_at),
+            reinterpret_cast<int32_t *>(scratch + free_at),
+            reinterpret_cast<uint32_t *>(scratch + ranks_at), static_cast<uint32_t>(rows)};
+}
+
+// A block alone where its shared memory holds the arrays and the table is
+// small, else the cluster.
+template <typename Args>
+void launch_plan(lro_context_t &context, const std::string &what, size_t array_bytes,
+                 uint64_t entries, const Args &args) {
+  if (array_bytes <= kPlanAloneBytes && entries <= kPlanAloneEntries) {
+    context.launch("ops_" + what + "_plan_alone", 1, kPlanThreadsAlone,
+                   static_cast<uint32_t>(array_bytes), args);
+  } else {
+    context.launch("ops_" + what + "_plan", kPlanBlocks, kPlanThreads, 0, args);
+  }
+}
+
 void pages_fork(lro_context_t &context, const lro_pages_fork_t &a) {
   MoveArgs moves{};
   const bool wide = pool_moves(a.pool, moves);
@@ -388,11 +417,10 @@ void pages_fork(lro_context_t &context, const lro_pages_fork_t &a) {
   require(a.rows_out == 0 || a.table.columns == 0 || a.table_out != a.table.pages,
           "table_out must not be the table");
   const size_t rows = a.rows_out, pages = a.pool.page_count;
-  const size_t moves_at = 256, rows_at = moves_at + aligned(sizeof(PageMove) * rows),
-               owners_at = rows_at + aligned(sizeof(ForkRow) * rows),
-               free_at = owners_at + aligned(4u * pages);
-  context.reserve(free_at + aligned(4u * pages));
-  auto *scratch = static_cast<unsigned char *>(context.scratch->data());
+  PlanArrays arrays{};
+  PageMove *list = nullptr;
+  uint32_t *list_count = nullptr;
+  plan_memory(context, rows, pages, rows, arrays, list, list_count);
   ForkArgs args{};
   args.table = table_of(a.table);
   args.lengths = a.lengths;
@@ -407,12 +435,11 @@ void pages_fork(lro_context_t &context, const lro_pages_fork_t &a) {
   args.capacity = a.table.columns * a.pool.page_size;
   args.page_count = a.pool.page_count;
   args.page = Divider::of(a.pool.page_size);
-  args.move_count = reinterpret_cast<uint32_t *>(scratch);
-  args.moves = reinterpret_cast<PageMove *>(scratch + moves_at);
-  args.owners = reinterpret_cast<uint32_t *>(scratch + owners_at);
-  args.free_pages = reinterpret_cast<int32_t *>(scratch + free_at);
-  args.rows = reinterpret_cast<ForkRow *>(scratch + rows_at);
-  context.launch("ops_fork_plan", kPlanBlocks, kPlanThreads, 0, args);
+  args.move_count = list_count;
+  args.moves = list;
+  args.arrays = arrays;
+  launch_plan(context, "fork", sizeof(ForkRow) * rows + 8u * pages,
+              uint64_t{a.rows_out} * a.table.columns, args);
   if (a.rows_out != 0 && a.pool.page_size > 1) { // pages of one token are never unfinished
     moves.moves = args.moves;
     moves.move_count = args.move_count;
@@ -430,10 +457,10 @@ void pages_compact(lro_context_t &context, const lro_pages_compact_t &a) {
   require(a.table_out != a.table.pages || a.table_out_row_stride == a.table.row_stride,
           "table_out is the table, with another stride");
   const size_t pages = a.pool.page_count;
-  const size_t moves_at = 256, marks_at = moves_at + aligned(sizeof(PageMove) * pages),
-               free_at = marks_at + aligned(4u * pages), ranks_at = free_at + aligned(4u * pages);
-  context.reserve(ranks_at + aligned(4u * pages));
-  auto *scratch = static_cast<unsigned char *>(context.scratch->data());
+  PlanArrays arrays{};
+  PageMove *list = nullptr;
+  uint32_t *list_count = nullptr;
+  plan_memory(context, 0, pages, pages, arrays, list, list_count);
   CompactArgs args{};
   args.table = table_of(a.table);
   args.held = a.held;
@@ -442,12 +469,10 @@ void pages_compact(lro_context_t &context, const lro_pages_compact_t &a) {
   args.status = a.status;
   args.page_count = a.pool.page_count;
   args.page_size = a.pool.page_size;
-  args.move_count = reinterpret_cast<uint32_t *>(scratch);
-  args.moves = reinterpret_cast<PageMove *>(scratch + moves_at);
-  args.marks = reinterpret_cast<uint32_t *>(scratch + marks_at);
-  args.free_pages = reinterpret_cast<int32_t *>(scratch + free_at);
-  args.ranks = reinterpret_cast<uint32_t *>(scratch + ranks_at);
-  context.launch("ops_compact_plan", kPlanBlocks, kPlanThreads, 0, args);
+  args.move_count = list_count;
+  args.moves = list;
+  args.arrays = arrays;
+  launch_plan(context, "compact", 12u * pages, uint64_t{a.table.rows} * a.table.columns, args);
   moves.moves = args.moves;
   moves.move_count = args.move_count;
   // A page moves only from above the live ones to below them: half the pool.

@@ -635,6 +635,36 @@ def test_compact(ops, torch, page, layout, kind, heads, dim):
         assert np.array_equal(keys.float().cpu().numpy(), want)
 
 
+def test_compact_many_rows_and_pages(ops, torch):
+    """More rows and pages than one block plans for; some pages held."""
+    rng = np.random.default_rng(4)
+    page, columns, count = 2, 60, 900
+    lengths = rng.integers(0, columns * page + 1, count).astype(np.int32)
+    used = int(sum(-(-lengths // page)))
+    for pages in (used + 25000, used):
+        table = random_table(rng, lengths, page, pages, columns, False)
+        held = (rng.random(pages) < 0.05).astype(np.uint8)
+        keys, values = page_pool(torch, "f16", 1, pages, page, 1, 2)
+        before = values.float().cpu().numpy()
+        live = np.zeros(pages, bool)
+        live[table[table >= 0]] = True
+        kept = held.astype(bool)
+        live &= ~kept
+        total = int((live | kept).sum())
+        sources = np.nonzero(live)[0]
+        sources = sources[sources >= total]
+        targets = np.nonzero(~live & ~kept)[0][:len(sources)]
+        want = before.copy()
+        want[:, targets] = before[:, sources]
+        place = np.arange(pages)
+        place[sources] = targets
+        got, status = ops.compact_pages(keys, values, torch.from_numpy(table).cuda(),
+                                        held=torch.from_numpy(held).cuda())
+        assert np.array_equal(got.cpu().numpy(), np.where(table >= 0, place[table.clip(0)], -1))
+        assert status.tolist() == [total, len(sources)]
+        assert np.array_equal(values.float().cpu().numpy(), want)
+
+
 def test_copy_pages(ops, torch):
     for kind, dim, layout in (("bf16", 8, "token"), ("f16", 2, "head"), ("f32", 3, "token")):
         keys, values = page_pool(torch, kind, 3, 20, 5, 2, dim, layout)
