@@ -234,12 +234,12 @@ LRRT_OPS_HD constexpr uint32_t beam_round(uint32_t element_bytes) {
 }
 constexpr uint32_t kBeamPool = 2048;              // candidates it holds
 constexpr uint32_t kBeamMaximumParts = 64;        // of a row
-constexpr uint32_t kBeamNotedRounds = 24;         // of a part
+constexpr uint32_t kBeamNotedRounds = 40;         // of a part
 constexpr uint32_t kBeamMaximumVocab = 1u << 21;
 static_assert(kBeamMaximumVocab <= kBeamNotedRounds * beam_round(4) *
                                        (kBeamPool / kBeamMaximumCount),
               "the parts of the longest row hold it");
-constexpr uint32_t kBeamSharedBytes = 46080;
+constexpr uint32_t kBeamSharedBytes = 62464;
 static_assert(kBeamMaximumCandidates <= kBeamPool, "a group's candidates fit the pool");
 
 struct Pair {

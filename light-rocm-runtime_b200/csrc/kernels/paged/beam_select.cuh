@@ -349,14 +349,16 @@ __device__ __forceinline__ void rank_beams(const BeamArgs &args, uint32_t group,
   }
 }
 
-// grid (parts, rows). Width elements a load.
-template <typename T, int Width>
+// grid (parts, rows). Parts begin on 16 bytes; the elements of a row before the
+// first such place, and after the last whole vector, are taken one by one.
+template <typename T>
 __device__ __forceinline__ void beam_select(const BeamArgs &args) {
   extern __shared__ __align__(16) unsigned char beam_memory[];
   BeamShared &shared = *reinterpret_cast<BeamShared *>(beam_memory);
   constexpr uint32_t kRound = beam_round(sizeof(T));
   constexpr int kEach = kRound / kBeamThreads; // elements of a thread and round
   constexpr int kPerWord = 4 / sizeof(T);
+  constexpr int Width = 16 / sizeof(T); // elements of a vector
   constexpr int kWords = kEach / kPerWord;
   using W = Words<T>;
   const uint32_t part = blockIdx.x, row = blockIdx.y;
@@ -365,8 +367,11 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
   const bool going = args.finished == nullptr || args.finished[row] == 0;
   if (going) {
     const T *logits = static_cast<const T *>(args.logits) + row * args.logits_stride;
-    const uint32_t begin = part * args.part_elements;
-    const uint32_t end = min(args.vocab, begin + args.part_elements);
+    const uint32_t skew =
+        min(static_cast<uint32_t>(-reinterpret_cast<uintptr_t>(logits) % 16u / sizeof(T)),
+            args.vocab); // elements before the row's first vector
+    const uint32_t begin = min(skew + part * args.part_elements, args.vocab);
+    const uint32_t end = min(args.vocab - begin, args.part_elements) + begin;
     auto index_of = [&](uint32_t round, int i) {
       return round + ((i / Width) * kBeamThreads + threadIdx.x) * Width + i % Width;
     };
@@ -381,15 +386,11 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
       for (int i = 0; i < kEach; i += Width) {
         const uint32_t index = index_of(round, i);
         if (index < whole) {
-          if constexpr (Width == 1) {
-            W::set(to[i / kPerWord], i % kPerWord, logits[index]);
-          } else {
-            const uint4 v = *reinterpret_cast<const uint4 *>(logits + index);
-            to[i / kPerWord] = v.x;
-            to[i / kPerWord + 1] = v.y;
-            to[i / kPerWord + 2] = v.z;
-            to[i / kPerWord + 3] = v.w;
-          }
+          const uint4 v = *reinterpret_cast<const uint4 *>(logits + index);
+          to[i / kPerWord] = v.x;
+          to[i / kPerWord + 1] = v.y;
+          to[i / kPerWord + 2] = v.z;
+          to[i / kPerWord + 3] = v.w;
         }
       }
     };
@@ -447,11 +448,17 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
       }
     }
 
-    // Elements past the last whole vector: one more round, of an element for
-    // each of the first threads.
+    // Elements before the first and past the last whole vector: one more round,
+    // of an element for each of the first threads.
+    auto odd_index = [&](uint32_t thread) -> uint32_t { // at `end` there is none
+      if (thread < Width) {
+        return part == 0 && thread < skew ? thread : end;
+      }
+      return min(whole + thread - Width, end);
+    };
     float odd = -INFINITY;
-    if (Width > 1 && threadIdx.x < end - whole) {
-      odd = to_float(logits[whole + threadIdx.x]);
+    if (threadIdx.x < 2u * Width && odd_index(threadIdx.x) != end) {
+      odd = to_float(logits[odd_index(threadIdx.x)]);
       odd = odd == odd ? odd : -INFINITY;
       largest = fmaxf(largest, odd);
       const float2 joined = join_sums(make_float2(top, sum), make_float2(odd * kLog2E, 1.0f));
@@ -489,8 +496,8 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
           begin + i * kRound + (lane / Width * kBeamThreads + thread) * Width + lane % Width;
       bool there = lane < kEach && index < whole;
       if (i == rounds) {
-        index = whole + thread;
-        there = lane == 0 && index < end;
+        index = odd_index(thread);
+        there = lane == 0 && index != end;
       }
       return there ? key_of(to_float(logits[index]), index) : kNoKey;
     };

@@ -78,19 +78,16 @@ LRRT_PLAN(compact_plan, CompactArgs)
 LRRT_MOVE(16, uint4)
 LRRT_MOVE(4, uint32_t)
 
-#define LRRT_BEAM(name, type, width)                                                              \
+#define LRRT_BEAM(name, type)                                                                     \
   extern "C" __global__ void __launch_bounds__(kBeamThreads, kBeamBlocksPerSm)                    \
       ops_beam_##name(const __grid_constant__ BeamArgs args) {                                    \
     wait_for_previous_launch();                                                                   \
-    beam_select<type, width>(args);                                                               \
+    beam_select<type>(args);                                                                      \
   }
 
-LRRT_BEAM(f32_x4, float, 4)
-LRRT_BEAM(f32_x1, float, 1)
-LRRT_BEAM(bf16_x8, __nv_bfloat16, 8)
-LRRT_BEAM(bf16_x1, __nv_bfloat16, 1)
-LRRT_BEAM(f16_x8, __half, 8)
-LRRT_BEAM(f16_x1, __half, 1)
+LRRT_BEAM(f32, float)
+LRRT_BEAM(bf16, __nv_bfloat16)
+LRRT_BEAM(f16, __half)
 
 extern "C" __global__ void __launch_bounds__(256)
     ops_zero(const __grid_constant__ ZeroArgs args) {

@@ -510,19 +510,17 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
   require(a.count == a.beams || (a.scores_out != a.scores &&
                                  (a.finished == nullptr || a.finished_out != a.finished)),
           "outputs may be inputs only where count = beams");
-  // Whole 16-byte vectors where every row starts on one.
-  const bool wide = multiple_of(a.logits, 16) && multiple_of(a.logits_row_stride, element, 16);
-  const uint32_t width = wide ? static_cast<uint32_t>(16u / element) : 1u;
   const size_t rows = size_t{a.groups} * a.beams;
-  // Parts of a row: the SM with most of them reads so many rounds one after
-  // another, and joining several parts takes about as long as eight.
+  // Parts of a row: the SM with most of them reads their rounds one after
+  // another; the fixed work of a part takes an SM about as long as four rounds,
+  // joining the parts of a row as eight.
   const uint32_t round = beam_round(static_cast<uint32_t>(element));
   const uint64_t rounds = ceil_div(a.vocab, round);
   const uint64_t most = std::min<uint64_t>({rounds, kBeamMaximumParts, kBeamPool / a.count});
   uint64_t parts = 1, least = ~uint64_t{0};
   for (uint64_t n = ceil_div(rounds, kBeamNotedRounds); n <= most; ++n) {
     const uint64_t cost =
-        ceil_div(rows * n, context.sms) * ceil_div(rounds, n) + (n > 1u ? 8u : 0u);
+        ceil_div(rows * n, context.sms) * (ceil_div(rounds, n) + 4u) + (n > 1u ? 8u : 0u);
     if (cost < least) {
       least = cost;
       parts = n;
@@ -559,7 +557,7 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
   args.row_log_sums = reinterpret_cast<float *>(scratch + log_sums_at);
   args.row_arrivals = counters;
   args.group_arrivals = counters + rows;
-  context.launch(std::string("ops_beam_") + type_name(a.type) + "_x" + std::to_string(width),
+  context.launch(std::string("ops_beam_") + type_name(a.type),
                  parts, kBeamThreads, kBeamSharedBytes, args, static_cast<uint32_t>(rows));
 }
 
