@@ -265,6 +265,23 @@ struct BeamArgs {
   uint32_t *group_arrivals; // [groups], likewise
 };
 
+// A beam search's bookkeeping before and after the operators of a step.
+struct BeamBeginArgs {
+  const int32_t *forked_table, *forked_lengths, *status; // of lro_pages_fork
+  int32_t *table;               // [rows][columns]
+  int32_t *lengths, *positions; // [rows]
+  uint32_t *missing_pages;
+  uint32_t rows, columns;
+};
+
+struct BeamEndArgs {
+  const int32_t *tokens, *parents;    // [rows], of lro_beam_select
+  uint32_t *next_tokens;              // [rows]
+  int32_t *all_tokens, *all_parents;  // [maximum_steps][rows]
+  uint32_t *step;
+  uint32_t rows, maximum_steps;
+};
+
 struct ZeroArgs {
   uint32_t *words;
   uint64_t count;

@@ -308,6 +308,39 @@ LRRT_API lr_status_t lrq_batch_position(lrq_batch_t *batch, uint32_t stream,
                                         uint32_t *position);
 
 /*
+ * Beam search over a paged KV cache (no counterpart in the reference, which
+ * decodes greedily). `groups` prompts with `beams` beams each (groups * beams
+ * rows, at most the prefill chunk size; at most 32 beams) decode as one batch;
+ * a beam holds up to `capacity` positions (at most the model's cache_capacity)
+ * in pages of `page_size` tokens that beams share until they part. Needs
+ * lrq_model_enable_prefill and the module of the paged-cache operators
+ * (paged_ops.cubin, include/lrrt_ops.h); destroy beam searches before
+ * re-enabling the prefill (lrq_model_destroy destroys any that remain).
+ *
+ * lrq_beam_search: the `beams` continuations by `steps` tokens of each prompt
+ *   with the highest sums of log-probabilities, as a search that keeps `beams`
+ *   of them at each step finds them. prompts holds the groups' tokens one after
+ *   another, counts[g] (at least 1) of each; counts[g] + steps <= capacity + 1.
+ *   tokens[(g * beams + k) * steps + i] and scores[g * beams + k] receive the
+ *   beams, best first. A beam that chose eos_token (UINT32_MAX: none) keeps its
+ *   score and goes on with that token; where fewer than `beams` continuations
+ *   exist, scores are -infinity and tokens -1. Equal scores are ordered as by
+ *   lro_beam_select. Waits for the device.
+ * Logits match single-stream decoding to FP32 rounding (GEMM summation order),
+ * not bit for bit.
+ */
+typedef struct lrq_beam_t lrq_beam_t;
+
+LRRT_API lr_status_t lrq_beam_create(lrq_model_t *model, const void *ops_image,
+                                     size_t ops_image_size, uint32_t groups, uint32_t beams,
+                                     uint32_t capacity, uint32_t page_size, uint32_t eos_token,
+                                     lrq_beam_t **beam);
+LRRT_API lr_status_t lrq_beam_destroy(lrq_beam_t *beam);
+LRRT_API lr_status_t lrq_beam_search(lrq_beam_t *beam, const uint32_t *prompts,
+                                     const uint32_t *counts, uint32_t steps, uint32_t path,
+                                     int32_t *tokens, float *scores);
+
+/*
  * End-to-end generate from host memory: copies the host hidden vector (or,
  * when hidden is NULL, stages the embedding of start_token) to the device,
  * runs the compiled path and copies the generated tokens back into `tokens`.

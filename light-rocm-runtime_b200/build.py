@@ -85,6 +85,14 @@ def build(verbose: bool = False) -> dict[str, Path]:
               *map(str, runtime_sources), "-o", str(runtime), "-ldl"], verbose)
     outputs["runtime"] = runtime
 
+    # Paged-cache operators (include/lrrt_ops.h).
+    ops = LIB / "liblrrt_ops.so"
+    ops_sources = [csrc / "ops" / "ops.cpp"]
+    if _stale(ops, ops_sources + headers + [runtime]):
+        _run([CXX, *CXXFLAGS, "-shared", "-fvisibility=hidden", *map(str, ops_sources), "-o",
+              str(ops), f"-L{LIB}", "-llrrt", "-Wl,-rpath,$ORIGIN"], verbose)
+    outputs["ops"] = ops
+
     driver = LIB / "liblrrt_qwen.so"
     driver_sources = sorted((csrc / "qwen").glob("*.cpp"))
     driver_headers = sorted((csrc / "qwen").glob("*.hpp"))
@@ -97,20 +105,12 @@ def build(verbose: bool = False) -> dict[str, Path]:
         _run([NVCC, *NVCCFLAGS, "-c", "-Xcompiler", "-fPIC,-fvisibility=hidden",
               str(static_top1), "-o", str(static_top1_object)], verbose)
     if _stale(driver, driver_sources + driver_headers + static_inputs +
-              [static_top1_object, runtime]):
+              [static_top1_object, runtime, ops]):
         _run([CXX, *CXXFLAGS, "-shared", "-fvisibility=hidden",
               *map(str, driver_sources), str(static_top1_object), "-o", str(driver),
-              f"-L{LIB}", "-llrrt", f"-L{CUDA_HOME / 'lib64'}", "-lcudart_static",
+              f"-L{LIB}", "-llrrt_ops", "-llrrt", f"-L{CUDA_HOME / 'lib64'}", "-lcudart_static",
               "-lrt", "-ldl", "-lpthread", "-Wl,-rpath,$ORIGIN"], verbose)
     outputs["driver"] = driver
-
-    # Paged-cache operators (include/lrrt_ops.h).
-    ops = LIB / "liblrrt_ops.so"
-    ops_sources = [csrc / "ops" / "ops.cpp"]
-    if _stale(ops, ops_sources + headers + [runtime]):
-        _run([CXX, *CXXFLAGS, "-shared", "-fvisibility=hidden", *map(str, ops_sources), "-o",
-              str(ops), f"-L{LIB}", "-llrrt", "-Wl,-rpath,$ORIGIN"], verbose)
-    outputs["ops"] = ops
 
     # The operators on torch tensors (lrrt_b200/ops.py): a Python extension.
     binding = LIB / "lrrt_ops_torch.so"

@@ -3,6 +3,7 @@
 // shape. The host library (csrc/ops/ops.cpp) picks them by name.
 #include "paged/attention.cuh"
 #include "paged/beam_select.cuh"
+#include "paged/beam_step.cuh"
 #include "paged/pages.cuh"
 #include "paged/rope_append.cuh"
 
@@ -88,6 +89,18 @@ LRRT_MOVE(4, uint32_t)
 LRRT_BEAM(f32, float)
 LRRT_BEAM(bf16, __nv_bfloat16)
 LRRT_BEAM(f16, __half)
+
+extern "C" __global__ void __launch_bounds__(256)
+    ops_beam_begin(const __grid_constant__ BeamBeginArgs args) {
+  wait_for_previous_launch();
+  beam_begin(args);
+}
+
+extern "C" __global__ void __launch_bounds__(256)
+    ops_beam_end(const __grid_constant__ BeamEndArgs args) {
+  wait_for_previous_launch();
+  beam_end(args);
+}
 
 extern "C" __global__ void __launch_bounds__(256)
     ops_zero(const __grid_constant__ ZeroArgs args) {

@@ -7,6 +7,7 @@
 
 #include "lm_head_top1_static.hpp"
 #include "batch.hpp"
+#include "beam.hpp"
 #include "prefill.hpp"
 #include "prefill_common.hpp"
 
@@ -311,6 +312,7 @@ struct lrq_model_t {
   std::unique_ptr<lrrt::qwen::prefill::Prefill> prefill;
   uint64_t weights_generation = 0;
   std::vector<lrq_batch_t *> batches; // live batched decoders (they use `prefill`)
+  std::vector<lrq_beam_t *> beams;    // live beam searches, likewise
 
   float *layer_weight(uint32_t layer, size_t offset) const {
     return static_cast<float *>(weights->data()) + size_t{layer} * layout.floats + offset;
@@ -969,6 +971,11 @@ struct lrq_batch_t {
   std::unique_ptr<lrrt::qwen::prefill::BatchDecoder> decoder;
 };
 
+struct lrq_beam_t {
+  lrq_model_t *model;
+  std::unique_ptr<lrrt::qwen::prefill::BeamSearch> search;
+};
+
 LRRT_API lr_status_t lrq_model_destroy(lrq_model_t *model) {
   return guarded("lrq_model_destroy", [&] {
     if (model == nullptr) {
@@ -978,6 +985,10 @@ LRRT_API lr_status_t lrq_model_destroy(lrq_model_t *model) {
       delete batch;
     }
     model->batches.clear();
+    for (lrq_beam_t *beam : model->beams) {
+      delete beam;
+    }
+    model->beams.clear();
     if (model->token_graph != nullptr) {
       model->device.synchronize();
       cudaGraphExecDestroy(model->token_graph);
@@ -1285,6 +1296,10 @@ LRRT_API lr_status_t lrq_model_enable_prefill(lrq_model_t *model, const void *mo
     if (!model->batches.empty()) {
       throw std::logic_error("destroy the model's batches before reloading the prefill module");
     }
+    if (!model->beams.empty()) {
+      throw std::logic_error(
+          "destroy the model's beam searches before reloading the prefill module");
+    }
     model->prefill.reset();
     model->prefill = std::make_unique<lrrt::qwen::prefill::Prefill>(
         model->device, module_image, module_image_size,
@@ -1429,6 +1444,55 @@ LRRT_API lr_status_t lrq_batch_position(lrq_batch_t *batch, uint32_t stream, uin
       throw std::invalid_argument("invalid batch position query");
     }
     *position = batch->decoder->position(stream);
+  });
+}
+
+LRRT_API lr_status_t lrq_beam_create(lrq_model_t *model, const void *ops_image,
+                                     size_t ops_image_size, uint32_t groups, uint32_t beams,
+                                     uint32_t capacity, uint32_t page_size, uint32_t eos_token,
+                                     lrq_beam_t **beam) {
+  return guarded("lrq_beam_create", [&] {
+    if (model == nullptr || ops_image == nullptr || ops_image_size == 0 || beam == nullptr) {
+      throw std::invalid_argument("null argument");
+    }
+    if (!model->prefill) {
+      throw std::logic_error("prefill is not enabled on this model");
+    }
+    auto created = std::make_unique<lrq_beam_t>();
+    created->model = model;
+    created->search = std::make_unique<lrrt::qwen::prefill::BeamSearch>(
+        *model->prefill, prefill_view(*model), ops_image, ops_image_size, groups, beams, capacity,
+        page_size, eos_token);
+    model->beams.push_back(created.get());
+    *beam = created.release();
+  });
+}
+
+LRRT_API lr_status_t lrq_beam_destroy(lrq_beam_t *beam) {
+  return guarded("lrq_beam_destroy", [&] {
+    if (beam == nullptr) {
+      throw std::invalid_argument("null beam search");
+    }
+    auto &list = beam->model->beams;
+    list.erase(std::remove(list.begin(), list.end(), beam), list.end());
+    delete beam;
+  });
+}
+
+LRRT_API lr_status_t lrq_beam_search(lrq_beam_t *beam, const uint32_t *prompts,
+                                     const uint32_t *counts, uint32_t steps, uint32_t path,
+                                     int32_t *tokens, float *scores) {
+  return guarded("lrq_beam_search", [&] {
+    if (beam == nullptr) {
+      throw std::invalid_argument("null beam search");
+    }
+    if (path != LRQ_PREFILL_SIMT && path != LRQ_PREFILL_TF32X3) {
+      throw std::invalid_argument("unknown prefill path");
+    }
+    lrq_model_t &m = *beam->model;
+    beam->search->search(prefill_view(m), prompts, counts, steps,
+                         static_cast<lrrt::qwen::prefill::Path>(path), m.weights_generation,
+                         tokens, scores);
   });
 }
 

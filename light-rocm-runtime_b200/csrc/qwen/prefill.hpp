@@ -44,6 +44,7 @@ struct ModelView {
 enum class Path : uint32_t { simt = 0, tf32x3 = 1 };
 
 class BatchDecoder;
+class BeamSearch;
 
 // (hi, lo) tensor maps of one GEMM operand: `wide` boxes for the
 // 128-row-band kernels (activations: 128 rows; weights: half a tile), and
@@ -77,6 +78,7 @@ public:
 
 private:
   friend class BatchDecoder;
+  friend class BeamSearch;
 
   // One layer's weights (gate_up_pair: the same rows in boxes of
   // kTcPairN / 2 for the prefill's pair tiles).

@@ -259,6 +259,9 @@ DRIVER_FUNCTIONS = {
     "lrq_batch_position": (u32, [vp, u32, P(u32)]),
     "lrq_batch_write_cache": (u32, [vp, u32, u32, u32, u32, vp, vp]),
     "lrq_batch_set_next": (u32, [vp, u32, u32, u32]),
+    "lrq_beam_create": (u32, [vp, vp, sz, u32, u32, u32, u32, u32, P(vp)]),
+    "lrq_beam_destroy": (u32, [vp]),
+    "lrq_beam_search": (u32, [vp, vp, vp, u32, u32, vp, vp]),
     "lrq_generate": (u32, [vp, vp, u32, u32, u32, u32, P(u32), P(RunState)]),
     "lrq_model_read": (u32, [vp, u32, u32, vp, sz]),
     "lrq_model_info": (u32, [vp, P(ModelInfo)]),

@@ -425,3 +425,42 @@ class Batch:
         N.check(N.driver().lrq_batch_position(self.handle, stream, C.byref(value)),
                 "lrq_batch_position")
         return value.value
+
+
+class Beam:
+    """Beam search over a paged KV cache (lrq_beam_* C ABI): `groups` prompts
+    with `beams` beams each, decoded as one batch on the GPU."""
+
+    def __init__(self, model: Model, groups: int, beams: int, capacity: int, page_size: int = 16,
+                 eos_token: int = NO_TOKEN, cubin: Optional[bytes] = None):
+        self.model = model
+        self.groups, self.beams = groups, beams
+        image = cubin if cubin is not None else N.OPS_CUBIN.read_bytes()
+        handle = C.c_void_p()
+        N.check(N.driver().lrq_beam_create(model.handle, image, len(image), groups, beams,
+                                           capacity, page_size, eos_token, C.byref(handle)),
+                "lrq_beam_create")
+        self.handle = handle
+
+    def close(self) -> None:
+        if self.handle:
+            N.check(N.driver().lrq_beam_destroy(self.handle), "lrq_beam_destroy")
+            self.handle = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def search(self, prompts, steps: int, path: int = PREFILL_TF32X3):
+        """(tokens [groups, beams, steps], scores [groups, beams]), best first."""
+        if len(prompts) != self.groups:
+            raise ValueError(f"{len(prompts)} prompts, not {self.groups}")
+        flat = np.array([int(t) for prompt in prompts for t in prompt], np.uint32)
+        counts = np.array([len(prompt) for prompt in prompts], np.uint32)
+        tokens = np.zeros((self.groups, self.beams, max(steps, 0)), np.int32)
+        scores = np.zeros((self.groups, self.beams), np.float32)
+        N.check(N.driver().lrq_beam_search(self.handle, _ptr(flat), _ptr(counts), steps, path,
+                                           _ptr(tokens), _ptr(scores)), "lrq_beam_search")
+        return tokens, scores
