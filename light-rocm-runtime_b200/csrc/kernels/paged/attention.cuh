@@ -823,7 +823,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     bool entered = false;
 #pragma unroll 1
     for (uint32_t step = 0; tile < end; ++step) {
-      if (!entered) {
+      if (!entered && step + 1u >= kStages) { // the first tiles are under way before
         begin_row(at.sequence, heads.first, heads.count);
         entered = true;
       }

@@ -511,16 +511,22 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
                                  (a.finished == nullptr || a.finished_out != a.finished)),
           "outputs may be inputs only where count = beams");
   const size_t rows = size_t{a.groups} * a.beams;
-  // Parts of a row: the SM with most of them reads their rounds one after
-  // another; the fixed work of a part takes an SM about as long as four rounds,
-  // joining the parts of a row as eight.
+  // Parts of a row, by the time of the SM with most of them. A round of 16 KB
+  // takes a block 0.9 us while no more than two share an SM (its latency), 1.1 us
+  // among three (their bandwidth); a part's fixed work is about four rounds,
+  // joining a row's parts 3 us and more with many of them. Measured with 256
+  // rows of 151936 bf16 logits: 1, 2, 3, 4 parts 32, 39, 39, 41 us; with 4 rows
+  // in f32: 10, 19, 38 parts 11.5, 10.9, 13.2 us.
   const uint32_t round = beam_round(static_cast<uint32_t>(element));
   const uint64_t rounds = ceil_div(a.vocab, round);
   const uint64_t most = std::min<uint64_t>({rounds, kBeamMaximumParts, kBeamPool / a.count});
   uint64_t parts = 1, least = ~uint64_t{0};
   for (uint64_t n = ceil_div(rounds, kBeamNotedRounds); n <= most; ++n) {
-    const uint64_t cost =
-        ceil_div(rows * n, context.sms) * (ceil_div(rounds, n) + 4u) + (n > 1u ? 8u : 0u);
+    const uint64_t blocks = ceil_div(rows * n, context.sms); // of the SM
+    const uint64_t cost = ceil_div(blocks, kBeamBlocksPerSm) *
+                              std::max<uint64_t>(90u, 37u * std::min<uint64_t>(blocks, 3u)) *
+                              (ceil_div(rounds, n) + 4u) +
+                          (n > 1u ? 300u + 8u * n : 0u);
     if (cost < least) {
       least = cost;
       parts = n;
