@@ -92,19 +92,20 @@ struct RopeAppendArgs {
 // Shared memory of an attention block: a ring of tiles for each of its warps,
 // and a partial state for each. A tile is 16 keys and values, or 32 of the
 // short rows of 128 bytes: 8 KB, and 16 KB for rows of 512 bytes. Eight warps
-// have three tiles each (two beside states of 16 heads), four where tiles are
-// large.
+// have three tiles each (two beside states of 16 heads); of the large tiles six
+// have two, four have three beside states of 256 elements.
 LRRT_OPS_HD constexpr uint32_t attention_tile_bytes(uint32_t row_bytes) {
   return row_bytes <= 256u ? 8192u : 16384u;
 }
 LRRT_OPS_HD constexpr uint32_t attention_tile_keys(uint32_t row_bytes) {
   return attention_tile_bytes(row_bytes) / (2u * row_bytes);
 }
-LRRT_OPS_HD constexpr uint32_t attention_warps(uint32_t row_bytes) {
-  return row_bytes <= 256u ? 8u : 4u;
+LRRT_OPS_HD constexpr uint32_t attention_warps(uint32_t dim, uint32_t row_bytes) {
+  return row_bytes <= 256u ? 8u : dim <= 128u ? 6u : 4u;
 }
-LRRT_OPS_HD constexpr uint32_t attention_stages(uint32_t heads) {
-  return heads > 8u ? 2u : 3u;
+LRRT_OPS_HD constexpr uint32_t attention_stages(uint32_t dim, uint32_t row_bytes,
+                                                uint32_t heads) {
+  return heads > 8u || attention_warps(dim, row_bytes) == 6u ? 2u : 3u;
 }
 // One partial state: the weighted values (rows padded against bank conflicts),
 // the maxima and the sums of a block's heads.
@@ -113,14 +114,15 @@ LRRT_OPS_HD constexpr uint32_t attention_state_floats(uint32_t dim, uint32_t hea
 }
 LRRT_OPS_HD constexpr uint32_t attention_shared_bytes(uint32_t dim, uint32_t row_bytes,
                                                       uint32_t heads) {
-  return attention_warps(row_bytes) *
-             (attention_stages(heads) * attention_tile_bytes(row_bytes) +
+  return attention_warps(dim, row_bytes) *
+             (attention_stages(dim, row_bytes, heads) * attention_tile_bytes(row_bytes) +
               4u * attention_state_floats(dim, heads)) +
          1024u;
 }
 static_assert(attention_shared_bytes(128, 256, 8) <= 232448u &&
                   attention_shared_bytes(128, 256, 16) <= 232448u &&
                   attention_shared_bytes(64, 256, 16) <= 232448u &&
+                  attention_shared_bytes(128, 512, 8) <= 232448u &&
                   attention_shared_bytes(256, 512, 8) <= 232448u,
               "a block's shared memory");
 // Tiles that a block takes at least, so that a short row is not split into

@@ -146,14 +146,14 @@ struct TileCursor {
 template <typename T, int Dim, int HeadTiles> class PagedAttention {
   static constexpr bool kWide = sizeof(T) == 4; // 32-bit elements
   static constexpr uint32_t kRowBytes = Dim * sizeof(T);
-  static constexpr uint32_t kWarps = attention_warps(kRowBytes);
+  static constexpr uint32_t kWarps = attention_warps(Dim, kRowBytes);
   static constexpr uint32_t kKeys = attention_tile_keys(kRowBytes);
   static constexpr uint32_t kChunks = kRowBytes / 16u; // 16-byte chunks of a row
   static constexpr uint32_t kRowsPerPass = 32u / kChunks;
   static constexpr uint32_t kKeyTiles = kKeys / 16u;
   static constexpr uint32_t kHeads = 8u * HeadTiles;
   static constexpr uint32_t kSteps = kRowBytes / 32u; // k steps of Q K^T (32 bytes of a row)
-  static constexpr uint32_t kStages = attention_stages(8u * HeadTiles);
+  static constexpr uint32_t kStages = attention_stages(Dim, kRowBytes, 8u * HeadTiles);
   static constexpr uint32_t kStageBytes = attention_tile_bytes(kRowBytes);
   static constexpr uint32_t kStateFloats = attention_state_floats(Dim, kHeads);
   static constexpr uint32_t kStateRow = Dim + 4u;           // floats of a head in a state

@@ -328,7 +328,7 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
   args.arrivals = static_cast<uint32_t *>(context.counters->data());
   context.launch(std::string("ops_attention_") + type_name(a.cache.type) + "_" +
                      std::to_string(dim) + "x" + std::to_string(heads),
-                 grid, 32u * attention_warps(row_bytes), attention_shared_bytes(dim, row_bytes, heads),
+                 grid, 32u * attention_warps(dim, row_bytes), attention_shared_bytes(dim, row_bytes, heads),
                  args);
 }
 
