@@ -227,12 +227,15 @@ struct MoveArgs {
 };
 
 constexpr uint32_t kBeamThreads = 256;
-constexpr uint32_t kBeamBlocksPerSm = 3;
+constexpr uint32_t kBeamBlocksPerSm = 2;
 constexpr uint32_t kBeamMaximumCount = 64;
 constexpr uint32_t kBeamMaximumCandidates = 2048; // beams * count
-// Elements that a block reads at a time: 16 KB.
+// A block reads a round of elements at a time, with four rounds under way: two
+// such blocks fill an SM's shared memory.
+constexpr uint32_t kBeamRoundBytes = 16384;
+constexpr uint32_t kBeamStages = 4;
 LRRT_OPS_HD constexpr uint32_t beam_round(uint32_t element_bytes) {
-  return 16384u / element_bytes;
+  return kBeamRoundBytes / element_bytes;
 }
 constexpr uint32_t kBeamPool = 2048;              // candidates it holds
 constexpr uint32_t kBeamMaximumParts = 64;        // of a row
@@ -241,7 +244,7 @@ constexpr uint32_t kBeamMaximumVocab = 1u << 21;
 static_assert(kBeamMaximumVocab <= kBeamNotedRounds * beam_round(4) *
                                        (kBeamPool / kBeamMaximumCount),
               "the parts of the longest row hold it");
-constexpr uint32_t kBeamSharedBytes = 62464;
+constexpr uint32_t kBeamSharedBytes = 111616;
 static_assert(kBeamMaximumCandidates <= kBeamPool, "a group's candidates fit the pool");
 
 struct Pair {

@@ -31,23 +31,6 @@
 
 namespace lrrt::ops {
 
-__device__ __forceinline__ uint32_t shared_address(const void *pointer) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(pointer));
-}
-
-// 16 bytes from global to shared memory; zeros where `valid` is false.
-__device__ __forceinline__ void copy_16(uint32_t to, uint64_t from, bool valid) {
-  const uint32_t bytes = valid ? 16u : 0u;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes)
-               : "memory");
-}
-__device__ __forceinline__ void commit_copies() {
-  asm volatile("cp.async.commit_group;" ::: "memory");
-}
-template <int Pending> __device__ __forceinline__ void wait_copies() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(Pending) : "memory");
-}
-
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t address) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -981,20 +964,18 @@ public:
     // Where this block is the last to leave its part of a row, it joins them.
     __syncthreads();
     if (threadIdx.x < 2u) {
-      __threadfence(); // what the barrier showed this thread, to the whole GPU
       const uint32_t i = threadIdx.x == 0 ? go_on[0] : go_on[1];
       uint32_t last = 0;
       if (i <= kWarps) {
         const Piece &piece = i == 0 ? firsts_[0] : lasts_[i - 1u];
         uint32_t *arrivals =
             args_.arrivals + size_t{piece.sequence} * args_.rows_per_sequence + piece.row;
-        last = atomicAdd(arrivals, 1u) + 1u == parts_of(piece, per_block) ? 1u : 0u;
+        last = arrive(arrivals) + 1u == parts_of(piece, per_block) ? 1u : 0u;
         if (last != 0) {
           *arrivals = 0;
         }
       }
       flags_[threadIdx.x] = last;
-      __threadfence();
     }
     __syncthreads();
 #pragma unroll 1

@@ -1,17 +1,21 @@
 // The best continuations over the beams of a group and the vocabulary.
 //
-// One pass over the logits. A block reads a part of a row, 16 KB a round. Each
-// thread keeps a running maximum and sum of exponentials (sums of disjoint
-// elements join as l1 e^(m1 - m) + l2 e^(m2 - m)), and notes the maximum of
-// each round. The threads' maxima give a floor that at least `count` elements
-// reach and few others; those few are read once more (from the caches, and only
-// where a noted maximum reaches the floor) and ranked. The last block of a row
-// joins the parts, the last row of a group ranks the beams' candidates by
-// score + logit - log sum.
+// One pass over the logits. A block reads a part of a row in rounds of 16 KB, four
+// of them under way by cp.async; every thread has its own elements copied, so
+// that rounds have no barriers. It keeps a running maximum and sum of
+// exponentials (sums of disjoint elements join as l1 e^(m1 - m) + l2 e^(m2 - m)),
+// and notes the maximum of each round. The threads' maxima give a floor that at
+// least `count` elements reach and few others; those few are read once more
+// (from the caches, and only where a noted maximum reaches the floor) and ranked.
+// The last block of a row joins the parts, the last row of a group ranks the
+// beams' candidates by score + logit - log sum.
 //
-// Bound by reading the logits once, for which an element must not cost more
-// than a handful of instructions, and by the fixed work of a part (floor,
-// ranking, joining) where there are few rows. The rounds have no barriers.
+// Bound by reading the logits once, by the exponentials (16 a clock and SM: 10 us
+// for the two rows of 151936 that the fullest SM has of 256), and by the fixed
+// work of a part (7 us to the end of the launch: floor, second reading, ranking,
+// joining) where there are few rows. Measured: 256 rows of 151936 logits in bf16,
+// 8 beams a group, 16 wanted, 24.3 us (3.2 TB/s; with two rounds under way in
+// registers 30.8 us); 200 rows in f32 29.3 us (4.2 TB/s); 4 rows in f32, 9.4 us.
 //
 // Pooled elements are 64-bit keys, the value's order in the upper half and the
 // complement of the index in the lower, so that no two are equal and the order
@@ -30,7 +34,10 @@ static_assert(kBeamShare == kBeamThreads && kBeamShare >= 2u * kBeamMaximumCount
 
 
 struct BeamShared {
-  uint64_t pool[kBeamPool];
+  union {
+    uint4 ring[kBeamStages][kBeamRoundBytes / 16u]; // rounds under way
+    uint64_t pool[kBeamPool];                       // after the last of them
+  };
   float noted[kBeamNotedRounds + 1][kBeamThreads]; // maximum of each round and thread
   uint64_t best[kBeamMaximumCount]; // the pool's best, falling, when it was last ranked
   uint64_t floors[kBeamWarps][32];
@@ -64,43 +71,6 @@ __device__ __forceinline__ uint64_t key_or_none(uint64_t key) {
 }
 
 __device__ __forceinline__ uint64_t larger(uint64_t a, uint64_t b) { return a > b ? a : b; }
-
-// The threads are split into `count` rounded up to a power of two classes,
-// each spread over the lanes and warps. The smallest of the classes' maxima is
-// no larger than the count-th largest of all elements; about
-// count * (1 + 1/2 + ... + 1/count) of them reach it where their order is
-// random. One barrier.
-template <typename T>
-__device__ __forceinline__ T class_floor(T mine, uint32_t count, BeamShared &shared) {
-  const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5u;
-  const bool two = count > 32u; // even and odd warps have classes of their own
-  uint32_t lanes = 1;
-  while (lanes < count && lanes < 32u) {
-    lanes <<= 1u;
-  }
-#pragma unroll
-  for (uint32_t offset = 16; offset != 0; offset >>= 1u) {
-    const T other = __shfl_xor_sync(kAllLanes, mine, offset);
-    mine = offset >= lanes && other > mine ? other : mine;
-  }
-  T *floors = reinterpret_cast<T *>(shared.floors);
-  floors[warp * 32u + lane] = mine;
-  __syncthreads();
-  T even = floors[lane], odd = floors[32u + lane];
-#pragma unroll
-  for (uint32_t w = 2; w < kBeamWarps; w += 2u) {
-    const T x = floors[w * 32u + lane], y = floors[(w + 1u) * 32u + lane];
-    even = x > even ? x : even;
-    odd = y > odd ? y : odd;
-  }
-  T least = two == (odd < even) ? odd : even; // of two classes the smaller, of one the larger
-#pragma unroll
-  for (uint32_t offset = 16; offset != 0; offset >>= 1u) {
-    const T other = __shfl_xor_sync(kAllLanes, least, offset);
-    least = other < least ? other : least;
-  }
-  return least;
-}
 
 // A floor that at least `count` elements reach, whose threads' maxima are
 // `mine`, and not many more: the threads form classes, at least four times
@@ -155,12 +125,11 @@ __device__ __forceinline__ uint64_t warp_largest(uint64_t key) {
 }
 
 // Puts the `count` largest of the pool's first `total` keys into `best`, falling,
-// kNoKey after the last: ranked by counting the larger ones; with more keys
-// than threads those below a floor are dropped first, and where that leaves too
-// many to count, the largest are taken one after another. The pool's contents
-// are lost. Begins and ends with a barrier.
+// kNoKey after the last: ranked by counting the larger ones. With more keys than
+// threads, those below the count-th largest of the threads' maxima are dropped
+// first: no more than `count` threads have keys that are left. The pool's
+// contents are lost. Begins and ends with a barrier.
 __device__ __noinline__ void rank_pool(uint32_t total, uint32_t count, BeamShared &shared) {
-  constexpr uint32_t kRanked = 1024; // as many are counted against one another
   const uint32_t thread = threadIdx.x;
   __syncthreads();
   if (total <= kBeamThreads) {
@@ -198,8 +167,20 @@ __device__ __noinline__ void rank_pool(uint32_t total, uint32_t count, BeamShare
   if (thread == 0) {
     shared.pooled = 0;
   }
-  const uint64_t floor = larger(kNoKey + 1u, class_floor(mine, count, shared));
-  if (mine >= floor) {
+  uint64_t *maxima = &shared.floors[0][0];
+  maxima[thread] = mine;
+  __syncthreads();
+  uint32_t larger_ones = 0;
+#pragma unroll 8
+  for (uint32_t j = 0; j < kBeamThreads; ++j) {
+    larger_ones += maxima[j] > mine ? 1u : 0u;
+  }
+  if (larger_ones + 1u == count) { // one thread: no two keys are equal
+    shared.best[0] = mine;
+  }
+  __syncthreads();
+  const uint64_t floor = shared.best[0];
+  if (larger_ones < count) {
 #pragma unroll
     for (uint32_t i = 0; i < kBeamWarps; ++i) {
       if (keys[i] >= floor) {
@@ -208,46 +189,17 @@ __device__ __noinline__ void rank_pool(uint32_t total, uint32_t count, BeamShare
     }
   }
   __syncthreads();
-  total = shared.pooled;
-  if (total <= kRanked) {
+  total = shared.pooled; // at least `count`
 #pragma unroll 1
-    for (uint32_t at = thread; at < total; at += kBeamThreads) {
-      const uint64_t key = shared.pool[at];
-      uint32_t rank = 0;
+  for (uint32_t at = thread; at < total; at += kBeamThreads) {
+    const uint64_t key = shared.pool[at];
+    uint32_t rank = 0;
 #pragma unroll 8
-      for (uint32_t j = 0; j < total; ++j) {
-        rank += shared.pool[j] > key ? 1u : 0u;
-      }
-      if (rank < count) {
-        shared.best[rank] = key_or_none(key);
-      }
+    for (uint32_t j = 0; j < total; ++j) {
+      rank += shared.pool[j] > key ? 1u : 0u;
     }
-    if (thread >= total && thread < count) {
-      shared.best[thread] = kNoKey;
-    }
-  } else {
-    uint64_t bound = ~uint64_t{0};
-#pragma unroll 1
-    for (uint32_t rank = 0; rank < count; ++rank) {
-      uint64_t best = kNoKey;
-#pragma unroll
-      for (uint32_t i = 0; i < kBeamWarps; ++i) {
-        best = keys[i] < bound ? larger(best, keys[i]) : best;
-      }
-      best = warp_largest(best);
-      __syncthreads();
-      if ((thread & 31u) == 0) {
-        shared.floors[thread >> 5u][0] = best;
-      }
-      __syncthreads();
-      bound = shared.floors[0][0];
-#pragma unroll
-      for (uint32_t w = 1; w < kBeamWarps; ++w) {
-        bound = larger(bound, shared.floors[w][0]);
-      }
-      if (thread == 0) {
-        shared.best[rank] = key_or_none(bound);
-      }
+    if (rank < count) {
+      shared.best[rank] = key_or_none(key);
     }
   }
   __syncthreads();
@@ -307,13 +259,10 @@ __device__ __forceinline__ bool arrive_last(uint32_t *counter, uint32_t blocks,
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    __threadfence(); // what the barrier showed this thread, to the whole GPU
-    const uint32_t before = atomicAdd(counter, 1u);
-    shared.last = before + 1u == blocks ? 1u : 0u;
+    shared.last = arrive(counter) + 1u == blocks ? 1u : 0u;
     if (shared.last != 0) {
       *counter = 0;
     }
-    __threadfence();
   }
   __syncthreads();
   return shared.last != 0;
@@ -398,21 +347,27 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
     };
     // A thread's elements of a round, -infinity past the last whole vector.
     const uint32_t whole = end - (end - begin) % Width;
-    auto load = [&](uint32_t(&to)[kWords], uint32_t round) {
-#pragma unroll
-      for (int k = 0; k < kWords; ++k) {
-        to[k] = W::kLeast;
-      }
+    auto load = [&](uint32_t stage, uint32_t round) {
 #pragma unroll
       for (int i = 0; i < kEach; i += Width) {
         const uint32_t index = index_of(round, i);
         if (index < whole) {
-          const uint4 v = *reinterpret_cast<const uint4 *>(logits + index);
-          to[i / kPerWord] = v.x;
-          to[i / kPerWord + 1] = v.y;
-          to[i / kPerWord + 2] = v.z;
-          to[i / kPerWord + 3] = v.w;
+          copy_16(shared_address(&shared.ring[stage][i / Width * kBeamThreads + threadIdx.x]),
+                  reinterpret_cast<uint64_t>(logits + index), true);
         }
+      }
+    };
+    auto read = [&](uint32_t(&to)[kWords], uint32_t stage, uint32_t round) {
+#pragma unroll
+      for (int i = 0; i < kEach; i += Width) {
+        uint4 v = shared.ring[stage][i / Width * kBeamThreads + threadIdx.x];
+        if (index_of(round, i) >= whole) {
+          v = make_uint4(W::kLeast, W::kLeast, W::kLeast, W::kLeast);
+        }
+        to[i / kPerWord] = v.x;
+        to[i / kPerWord + 1] = v.y;
+        to[i / kPerWord + 2] = v.z;
+        to[i / kPerWord + 3] = v.w;
       }
     };
     float top = -INFINITY, sum = 0.0f; // as join_sums takes them
@@ -428,11 +383,12 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
       largest = fmaxf(largest, most);
       const float now = fmaxf(top, most * kLog2E);
       const float base = now == -INFINITY ? 0.0f : now;
-      float terms = 0.0f;
+      float each[4] = {}; // four sums at a time
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        terms += exp2_fast(fmaf(W::value(from[i / kPerWord], i % kPerWord), kLog2E, -base));
+        each[i % 4] += exp2_fast(fmaf(W::value(from[i / kPerWord], i % kPerWord), kLog2E, -base));
       }
+      float terms = (each[0] + each[1]) + (each[2] + each[3]);
       if (terms != terms) { // there is a NaN
         terms = 0.0f;
 #pragma unroll 1
@@ -445,28 +401,29 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
       sum = sum * exp2_fast(top - base) + terms;
       top = now;
     };
-    // Two rounds are under way: a buffer is filled again once it is used up.
-    constexpr uint32_t kAhead = 2;
-    uint32_t buffers[kAhead][kWords];
+    // Each thread has its own elements copied, so that rounds need no barrier;
+    // a stage is filled again once its elements are in registers.
     const uint32_t rounds = (whole - begin + kRound - 1u) / kRound;
 #pragma unroll
-    for (uint32_t i = 0; i < kAhead; ++i) {
+    for (uint32_t i = 0; i < kBeamStages; ++i) {
       if (i < rounds) {
-        load(buffers[i], begin + i * kRound);
+        load(i, begin + i * kRound);
       }
+      commit_copies();
     }
+    uint32_t stage = 0;
 #pragma unroll 1
-    for (uint32_t number = 0; number < rounds; number += kAhead) {
-#pragma unroll
-      for (uint32_t i = 0; i < kAhead; ++i) {
-        if (number + i < rounds) {
-          const uint32_t round = begin + (number + i) * kRound;
-          take(buffers[i], round, number + i);
-          if (number + i + kAhead < rounds) {
-            load(buffers[i], round + kAhead * kRound);
-          }
-        }
+    for (uint32_t number = 0; number < rounds; ++number) {
+      const uint32_t round = begin + number * kRound;
+      uint32_t words[kWords];
+      wait_copies<kBeamStages - 1>();
+      read(words, stage, round);
+      if (number + kBeamStages < rounds) {
+        load(stage, round + kBeamStages * kRound);
       }
+      commit_copies();
+      take(words, round, number);
+      stage = stage + 1u == kBeamStages ? 0u : stage + 1u;
     }
 
     // Elements before the first and past the last whole vector: one more round,
@@ -493,6 +450,7 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
     // four such reads at a time.
     static_assert(kEach <= 32, "a lane per element");
     static_assert((kBeamNotedRounds + 1u) * kBeamThreads <= 65536u, "a listed round is 16 bits");
+    static_assert(kBeamNotedRounds + 1u <= 64u, "a bit per round");
     constexpr uint32_t kListed = 2u * kBeamPool, kPooled = kBeamPool / 2u;
     auto *list = reinterpret_cast<uint16_t *>(shared.pool + kPooled); // the pool's other half
     if (threadIdx.x == 0) {
@@ -501,12 +459,17 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
     }
     float floor = count_floor(largest, args.count, shared);
     uint64_t least_key = uint64_t{order_of(floor)} << 32; // the lowest that enters
+    uint64_t reaching = 0; // this thread's rounds
 #pragma unroll 4
     for (uint32_t i = 0; i <= rounds; ++i) {
-      if (shared.noted[i][threadIdx.x] >= floor) {
-        const uint32_t at = atomicAdd(&shared.listed, 1u);
+      reaching |= uint64_t{shared.noted[i][threadIdx.x] >= floor} << i;
+    }
+    if (reaching != 0) {
+      uint32_t at = atomicAdd(&shared.listed, static_cast<uint32_t>(__popcll(reaching)));
+#pragma unroll 1
+      for (; reaching != 0; reaching &= reaching - 1u, ++at) {
         if (at < kListed) {
-          list[at] = static_cast<uint16_t>(i * kBeamThreads + threadIdx.x);
+          list[at] = static_cast<uint16_t>((__ffsll(reaching) - 1) * kBeamThreads + threadIdx.x);
         }
       }
     }

@@ -159,6 +159,35 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+__device__ __forceinline__ uint32_t shared_address(const void *pointer) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(pointer));
+}
+
+// 16 bytes from global to shared memory; zeros where `valid` is false.
+__device__ __forceinline__ void copy_16(uint32_t to, uint64_t from, bool valid) {
+  const uint32_t bytes = valid ? 16u : 0u;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void commit_copies() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int Pending> __device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(Pending) : "memory");
+}
+
+// Counts a block in, by one thread after a barrier of its threads: what they
+// wrote before is seen by the threads that pass a barrier with the one that
+// counted in later. Returns how many were there before.
+__device__ __forceinline__ uint32_t arrive(uint32_t *counter) {
+  uint32_t before;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+               : "=r"(before)
+               : "l"(__cvta_generic_to_global(counter))
+               : "memory");
+  return before;
+}
+
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -511,22 +511,25 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
                                  (a.finished == nullptr || a.finished_out != a.finished)),
           "outputs may be inputs only where count = beams");
   const size_t rows = size_t{a.groups} * a.beams;
-  // Parts of a row, by the time of the SM with most of them. A round of 16 KB
-  // takes a block 0.9 us while no more than two share an SM (its latency), 1.1 us
-  // among three (their bandwidth); a part's fixed work is about four rounds,
-  // joining a row's parts 3 us and more with many of them. Measured with 256
-  // rows of 151936 bf16 logits: 1, 2, 3, 4 parts 32, 39, 39, 41 us; with 4 rows
-  // in f32: 10, 19, 38 parts 11.5, 10.9, 13.2 us.
+  // Parts of a row, by the time of the SM with most of them, in units of 10 ns. A
+  // round of 16 KB takes a block 0.42 us of 16-bit elements and 0.3 us of 32-bit
+  // ones where it has its SM alone, 0.7 and 0.48 us where two share it; a part's
+  // fixed work (floor, ranking) 4.2 us alone and 4.8 us beside another; joining
+  // a row's parts 2.5 us and a little for each. Measured, 151936 logits: 256 rows in
+  // bf16 1, 2, 3 parts 25, 33, 38 us; 96 rows in f32 1, 2, 3, 4 parts 21, 21, 20.7,
+  // 27 us; 32 rows in bf16 1, 2, 4, 5, 8 parts 17, 15, 13, 14.5, 13.6 us; 4 rows in
+  // f32 4, 8, 20, 38 parts 11.4, 10.0, 9.4, 10.7 us.
   const uint32_t round = beam_round(static_cast<uint32_t>(element));
   const uint64_t rounds = ceil_div(a.vocab, round);
   const uint64_t most = std::min<uint64_t>({rounds, kBeamMaximumParts, kBeamPool / a.count});
+  const uint64_t alone_round = element == 4u ? 30u : 42u, shared_round = element == 4u ? 48u : 70u;
   uint64_t parts = 1, least = ~uint64_t{0};
   for (uint64_t n = ceil_div(rounds, kBeamNotedRounds); n <= most; ++n) {
     const uint64_t blocks = ceil_div(rows * n, context.sms); // of the SM
-    const uint64_t cost = ceil_div(blocks, kBeamBlocksPerSm) *
-                              std::max<uint64_t>(90u, 37u * std::min<uint64_t>(blocks, 3u)) *
-                              (ceil_div(rounds, n) + 4u) +
-                          (n > 1u ? 300u + 8u * n : 0u);
+    const uint64_t waves = ceil_div(blocks, kBeamBlocksPerSm);
+    const uint64_t cost = waves * ((blocks > 1u ? shared_round : alone_round) * ceil_div(rounds, n) +
+                                   (blocks > 1u ? 480u : 420u)) +
+                          (n > 1u ? 250u + 4u * n : 0u);
     if (cost < least) {
       least = cost;
       parts = n;
