@@ -93,7 +93,8 @@ struct RopeAppendArgs {
 // and a partial state for each. A tile is 16 keys and values, or 32 of the
 // short rows of 128 bytes: 8 KB, and 16 KB for rows of 512 bytes. Eight warps
 // have three tiles each (two beside states of 16 heads); of the large tiles six
-// have two, four have three beside states of 256 elements.
+// have two (four with three: 206 us instead of 179 for 64 sequences of up to 8192
+// keys, 4 heads of 128 in f32), four have three beside states of 256 elements.
 LRRT_OPS_HD constexpr uint32_t attention_tile_bytes(uint32_t row_bytes) {
   return row_bytes <= 256u ? 8192u : 16384u;
 }
@@ -125,14 +126,21 @@ static_assert(attention_shared_bytes(128, 256, 8) <= 232448u &&
                   attention_shared_bytes(128, 512, 8) <= 232448u &&
                   attention_shared_bytes(256, 512, 8) <= 232448u,
               "a block's shared memory");
-// Tiles that a block takes at least, so that a short row is not split into
-// more partial states than its tiles are worth.
-constexpr uint32_t kAttentionMinimumTiles = 8;
-// Where no row has more tiles than this, blocks take whole rows: there are
-// states to join in shared memory only.
-constexpr uint32_t kAttentionWholeTiles = 32;
+// Places that a block takes at least, so that a short row is not split into more
+// partial states than its tiles are worth. Measured (2000 bf16 keys of 8 heads of
+// 128, group of 4): at least 4, 8, 16 of them 8.9, 10.6, 10.9 us.
+constexpr uint32_t kAttentionMinimumTiles = 4;
+// Where no row has more tiles than this, blocks take whole rows, so that states
+// are joined in shared memory only: the first of these with few rows, the
+// second where there are at least half as many as blocks. Measured, whole rows
+// and split ones: 8 rows of 10 tiles 7.4 and 8.5 us; 8 rows of 19 tiles 8.7 and
+// 7.5 us; 128 rows of 31 tiles 11.7 and 13.3 us; 64 rows of 64 tiles 20.7 and
+// 16.2 us.
+constexpr uint32_t kAttentionWholeTilesFew = 16;
+constexpr uint32_t kAttentionWholeTilesMany = 32;
 // What a row costs a warp besides its tiles (its queries, and its end), in
-// tiles.
+// tiles. Measured with 0, 1, 3: 64 sequences of up to 900 keys 29.1, 23.0, 23.7
+// us; of up to 8192 keys 137, 135, 135 us; 128 of up to 200 keys 21.6, 17.8, 18.6 us.
 constexpr uint32_t kAttentionRowCost = 1;
 
 struct PagedAttentionArgs {

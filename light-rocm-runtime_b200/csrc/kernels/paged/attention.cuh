@@ -921,8 +921,10 @@ public:
         max((total + gridDim.x - 1u) / gridDim.x, kAttentionMinimumTiles);
     uint32_t begin = min(blockIdx.x * per_block, total);
     uint32_t end = min(begin + per_block, total);
-    if (share == 1u &&
-        most <= (kAttentionWholeTiles + kAttentionRowCost) * args_.rows_per_sequence) {
+    const uint32_t whole_tiles =
+        2u * args_.table.rows * args_.rows_per_sequence >= gridDim.x ? kAttentionWholeTilesMany
+                                                                     : kAttentionWholeTilesFew;
+    if (share == 1u && most <= (whole_tiles + kAttentionRowCost) * args_.rows_per_sequence) {
       begin = row_boundary(begin, total, share);
       end = row_boundary(end, total, share);
     }
