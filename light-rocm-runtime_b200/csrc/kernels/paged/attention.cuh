@@ -6,7 +6,7 @@
 //
 // Bound by reading the cache once. What the layout does about that:
 //  - Every warp streams its own tiles (8 or 16 KB of keys and values) through
-//    shared-memory stages filled by cp.async, so a block keeps about 128 KB in
+//    shared-memory stages filled by cp.async, so a block keeps 128 to 192 KB in
 //    flight without a barrier between its warps. Rows are gathered through the
 //    page table, whose entries are read one tile ahead.
 //  - The query heads of one key-value head share each row that is read: scores
@@ -24,6 +24,13 @@
 //    a row lies in several blocks through the workspace by the last of them to
 //    arrive. Pieces are joined in their order, so that results do not depend on
 //    timing.
+//
+// Measured (cache reads at 6.5 TB/s take the time in brackets): 64 ragged
+// sequences of up to 8192 keys, 32 heads over 8 of 128 elements in bf16, 135 us
+// (122); two of about 123000 keys with capped scores 49 us (38); pages of one token
+// 165 us. Few keys are bound by latency (launch, lengths, page numbers, first
+// tile, joining): 32 sequences of 1152, 14 heads over 2 of 64 in f32, 16.2 us
+// (5.5); one of 160, 7.8 us.
 #ifndef LRRT_PAGED_ATTENTION_CUH_
 #define LRRT_PAGED_ATTENTION_CUH_
 

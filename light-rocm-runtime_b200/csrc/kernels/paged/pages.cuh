@@ -2,13 +2,16 @@
 //
 // A plan kernel works out the new tables and a list of page moves: one block
 // with its working arrays in shared memory where they fit, else a cluster of
-// eight with them in the workspace. A copy kernel over the whole GPU then moves the rows of
-// every layer. Which pages are free follows from the tables alone, so no
+// eight with them in the workspace. A copy kernel over the whole GPU then moves
+// the rows of every layer. Which pages are free follows from the tables alone, so no
 // reference counts are kept that could drift from them. Every choice is the
 // lowest number, so the results do not depend on the order of threads.
 //
 // The plan is bound by latency (a few dependent reads of small tables between
-// barriers), the copy by memory bandwidth.
+// barriers), the copy by memory bandwidth. Measured, both launches: forks of 32
+// beams over 24 layers of 2 heads of 64 in f32 8.0 us (0.9 us of copies), of 128
+// beams over 16 layers of 8 heads of 128 in bf16 24.5 us (15.5 of copies, 4.1
+// TB/s over all); a compaction that moves 230 MB 77.5 us (5.9 TB/s).
 #ifndef LRRT_PAGED_PAGES_CUH_
 #define LRRT_PAGED_PAGES_CUH_
 

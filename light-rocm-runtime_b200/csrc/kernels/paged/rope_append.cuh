@@ -8,7 +8,12 @@
 // copied, and has its loads under way before it knows the token's place.
 // Neighbouring threads take neighbouring columns, so rows are read and written
 // in whole lines. Value heads come after all query and key heads: blocks do
-// one or the other.
+// one or the other. More vectors a thread (four heads' with the same angles) left
+// fewer loads under way and took 124 us where this takes 72.
+//
+// Measured, 32 heads over 8 of 128 elements in bf16: 16384 tokens 72 us (5.7 TB/s);
+// 14 heads over 2 of 64 in f32, one token for each of 32 sequences: 2.1 us, a
+// launch's latency.
 #ifndef LRRT_PAGED_ROPE_APPEND_CUH_
 #define LRRT_PAGED_ROPE_APPEND_CUH_
 
