@@ -95,6 +95,10 @@ struct RopeAppendArgs {
 // have three tiles each (two beside states of 16 heads); of the large tiles six
 // have two (four with three: 206 us instead of 179 for 64 sequences of up to 8192
 // keys, 4 heads of 128 in f32), four have three beside states of 256 elements.
+// Rows of 96 elements (for heads of 65 to 96) lie in the places of 128.
+LRRT_OPS_HD constexpr uint32_t attention_row_bytes(uint32_t dim, uint32_t element_bytes) {
+  return (dim == 96u ? 128u : dim) * element_bytes;
+}
 LRRT_OPS_HD constexpr uint32_t attention_tile_bytes(uint32_t row_bytes) {
   return row_bytes <= 256u ? 8192u : 16384u;
 }

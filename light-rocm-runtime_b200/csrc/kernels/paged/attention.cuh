@@ -135,14 +135,14 @@ struct TileCursor {
 
 template <typename T, int Dim, int HeadTiles> class PagedAttention {
   static constexpr bool kWide = sizeof(T) == 4; // 32-bit elements
-  static constexpr uint32_t kRowBytes = Dim * sizeof(T);
+  static constexpr uint32_t kRowBytes = attention_row_bytes(Dim, sizeof(T)); // in a tile
   static constexpr uint32_t kWarps = attention_warps(Dim, kRowBytes);
   static constexpr uint32_t kKeys = attention_tile_keys(kRowBytes);
   static constexpr uint32_t kChunks = kRowBytes / 16u; // 16-byte chunks of a row
   static constexpr uint32_t kRowsPerPass = 32u / kChunks;
   static constexpr uint32_t kKeyTiles = kKeys / 16u;
   static constexpr uint32_t kHeads = 8u * HeadTiles;
-  static constexpr uint32_t kSteps = kRowBytes / 32u; // k steps of Q K^T (32 bytes of a row)
+  static constexpr uint32_t kSteps = Dim * sizeof(T) / 32u; // of Q K^T (32 bytes of a row)
   static constexpr uint32_t kStages = attention_stages(Dim, kRowBytes, 8u * HeadTiles);
   static constexpr uint32_t kStageBytes = attention_tile_bytes(kRowBytes);
   static constexpr uint32_t kStateFloats = attention_state_floats(Dim, kHeads);
@@ -250,8 +250,10 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
           __shfl_sync(kAllLanes, reinterpret_cast<uint64_t>(value), row) + offset;
       const bool valid = (wanted >> row & 1u) != 0;
       const uint32_t at = keys + swizzled(row, chunk);
-      copy_16(at, key_row, valid);
-      copy_16(at + kStageBytes / 2u, value_row, valid);
+      if (chunk < Dim * sizeof(T) / 16u) {
+        copy_16(at, key_row, valid);
+        copy_16(at + kStageBytes / 2u, value_row, valid);
+      }
     }
   }
 
@@ -330,6 +332,16 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
                                           uint32_t first_head, uint32_t heads) {
     const uint32_t keys = ring_ + stage * kStageBytes;
     const uint32_t values = keys + kStageBytes / 2u;
+    float slope[HeadTiles][2]; // under way before the products; 0 without a bias
+#pragma unroll
+    for (int n = 0; n < HeadTiles; ++n) {
+#pragma unroll
+      for (uint32_t i = 0; i < 2u; ++i) {
+        const uint32_t head = n * 8u + (lane_ & 3u) * 2u + i;
+        slope[n][i] =
+            args_.slopes != nullptr && head < heads ? args_.slopes[first_head + head] : 0.0f;
+      }
+    }
     float score[HeadTiles][kKeyTiles][4];
 #pragma unroll
     for (uint32_t m = 0; m < kKeyTiles; ++m) {
@@ -374,18 +386,11 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
       }
     }
     const uint32_t seen = seen_[stage];
-    const float to_base_2 = args_.softcap > 0.0f ? args_.softcap * kLog2E : args_.scale * kLog2E;
-    const float to_cap = args_.softcap > 0.0f ? args_.scale / args_.softcap : 0.0f;
+    const bool capped = args_.softcap > 0.0f;
+    const float to_base_2 = (capped ? args_.softcap : args_.scale) * kLog2E;
+    const float to_cap = capped ? args_.scale / args_.softcap : 0.0f;
 #pragma unroll
     for (int n = 0; n < HeadTiles; ++n) {
-      float slope[2] = {0.0f, 0.0f};
-      if (args_.slopes != nullptr) {
-#pragma unroll
-        for (uint32_t i = 0; i < 2u; ++i) {
-          const uint32_t head = n * 8u + (lane_ & 3u) * 2u + i;
-          slope[i] = head < heads ? args_.slopes[first_head + head] * kLog2E : 0.0f;
-        }
-      }
       float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (uint32_t m = 0; m < kKeyTiles; ++m) {
@@ -393,10 +398,19 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
         for (int i = 0; i < 4; ++i) {
           const uint32_t key = m * 16u + (i / 2) * 8u + lane_ / 4u;
           float s = score[n][m][i];
-          s = args_.softcap > 0.0f ? tanhf(s * to_cap) * to_base_2 : s * to_base_2;
+          if (!capped) {
+            s *= to_base_2;
+          } else if constexpr (kWide) {
+            s = tanhf(s * to_cap) * to_base_2;
+          } else {
+            // tanh x = 1 - 2 / (1 + e^2x): near 0 only the absolute error is
+            // small, 2e-7 of the cap, which outputs of 16 bits do not show.
+            s = fmaf(reciprocal_fast(1.0f + exp2_fast(s * (2.0f * kLog2E * to_cap))),
+                     -2.0f * to_base_2, to_base_2);
+          }
           if (args_.slopes != nullptr) {
             const int32_t distance = static_cast<int32_t>(end - 1u - first_key - key);
-            s -= slope[i % 2] * static_cast<float>(distance);
+            s -= slope[n][i % 2] * kLog2E * static_cast<float>(distance);
           }
           s = (seen >> key & 1u) != 0 ? s : -INFINITY;
           score[n][m][i] = s;

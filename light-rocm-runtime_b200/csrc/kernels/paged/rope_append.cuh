@@ -5,7 +5,7 @@
 // Bound by memory: every input is read once and every output written once
 // (the cosine and sine rows come from the caches, a token's heads share them).
 // A thread takes a vector of each half of a head's pairs, or a vector that is
-// copied, and has its loads under way before it knows the token's place.
+// copied (CopyWidth elements: wider where only the halves are odd), and has its loads under way before it knows the token's place.
 // Neighbouring threads take neighbouring columns, so rows are read and written
 // in whole lines. Value heads come after all query and key heads: blocks do
 // one or the other. More vectors a thread (four heads' with the same angles) left
@@ -61,7 +61,7 @@ __device__ __forceinline__ void append_values(const RopeAppendArgs &args, uint32
   }
 }
 
-template <typename T, int Width, bool Interleaved>
+template <typename T, int Width, int CopyWidth, bool Interleaved>
 __device__ __forceinline__ void rope_append(const RopeAppendArgs &args) {
   using V = WordVector<T, Width>;
   using W = Words<T>;
@@ -70,7 +70,7 @@ __device__ __forceinline__ void rope_append(const RopeAppendArgs &args) {
   if (blockIdx.x >= turned_blocks) {
     const uint32_t item = (blockIdx.x - turned_blocks) * kRopeThreads + threadIdx.x;
     if (item < args.value_items) {
-      append_values<T, Width>(args, item);
+      append_values<T, CopyWidth>(args, item);
     }
     return;
   }
@@ -88,7 +88,7 @@ __device__ __forceinline__ void rope_append(const RopeAppendArgs &args) {
   const bool turns = unit < turned;
   const uint32_t pair = unit * Width; // first of the pairs
   // The elements: of the pairs' first and second halves, or past the pairs.
-  uint32_t at = args.rotary_dim + (unit - turned) * Width, at_second = at;
+  uint32_t at = args.rotary_dim + (unit - turned) * CopyWidth, at_second = at;
   if (turns) {
     at = Interleaved ? 2u * pair : pair;
     at_second = Interleaved ? at + Width : at + half;
@@ -97,7 +97,12 @@ __device__ __forceinline__ void rope_append(const RopeAppendArgs &args) {
                                args.k.offset(token, head - args.heads)
                          : static_cast<const T *>(args.q.data) + args.q.offset(token, head);
   V x[2];
-  x[0].load(from + at);
+  WordVector<T, CopyWidth> copied;
+  if (CopyWidth == Width || turns) {
+    x[0].load(from + at);
+  } else {
+    copied.load(from + at);
+  }
   if (turns) {
     x[1].load(from + at_second);
   }
@@ -115,6 +120,7 @@ __device__ __forceinline__ void rope_append(const RopeAppendArgs &args) {
     if (!place.valid) { // padding
       x[0] = V{};
       x[1] = V{};
+      copied = {};
     }
   }
   if (turns && place.valid) {
@@ -170,7 +176,11 @@ __device__ __forceinline__ void rope_append(const RopeAppendArgs &args) {
       }
     }
   }
-  x[0].store(to + at);
+  if (CopyWidth == Width || turns) {
+    x[0].store(to + at);
+  } else {
+    copied.store(to + at);
+  }
   if (turns) {
     x[1].store(to + at_second);
   }

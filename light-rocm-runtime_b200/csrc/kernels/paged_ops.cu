@@ -9,26 +9,28 @@
 
 using namespace lrrt::ops;
 
-#define LRRT_ROPE(name, type, width)                                                              \
+#define LRRT_ROPE(name, type, width, copy_width)                                                  \
   extern "C" __global__ void __launch_bounds__(kRopeThreads)                                      \
       ops_rope_half_##name(const __grid_constant__ RopeAppendArgs args) {                         \
     wait_for_previous_launch();                                                                   \
-    rope_append<type, width, false>(args);                                                        \
+    rope_append<type, width, copy_width, false>(args);                                            \
   }                                                                                               \
   extern "C" __global__ void __launch_bounds__(kRopeThreads)                                      \
       ops_rope_pairs_##name(const __grid_constant__ RopeAppendArgs args) {                        \
     wait_for_previous_launch();                                                                   \
-    rope_append<type, width, true>(args);                                                         \
+    rope_append<type, width, copy_width, true>(args);                                             \
   }
 
-LRRT_ROPE(f32_x4, float, 4)
-LRRT_ROPE(f32_x1, float, 1)
-LRRT_ROPE(bf16_x8, __nv_bfloat16, 8)
-LRRT_ROPE(bf16_x4, __nv_bfloat16, 4)
-LRRT_ROPE(bf16_x1, __nv_bfloat16, 1)
-LRRT_ROPE(f16_x8, __half, 8)
-LRRT_ROPE(f16_x4, __half, 4)
-LRRT_ROPE(f16_x1, __half, 1)
+LRRT_ROPE(f32_x4, float, 4, 4)
+LRRT_ROPE(f32_x1, float, 1, 1)
+LRRT_ROPE(bf16_x8, __nv_bfloat16, 8, 8)
+LRRT_ROPE(bf16_x4x8, __nv_bfloat16, 4, 8)
+LRRT_ROPE(bf16_x4, __nv_bfloat16, 4, 4)
+LRRT_ROPE(bf16_x1, __nv_bfloat16, 1, 1)
+LRRT_ROPE(f16_x8, __half, 8, 8)
+LRRT_ROPE(f16_x4x8, __half, 4, 8)
+LRRT_ROPE(f16_x4, __half, 4, 4)
+LRRT_ROPE(f16_x1, __half, 1, 1)
 
 #define LRRT_ATTENTION(name, type, dim, head_tiles)                                               \
   extern "C" __global__ void __launch_bounds__(PagedAttention<type, dim, head_tiles>::kThreads, 1) \
@@ -40,14 +42,19 @@ LRRT_ROPE(f16_x1, __half, 1)
 
 LRRT_ATTENTION(f32_64x8, float, 64, 1)
 LRRT_ATTENTION(f32_64x16, float, 64, 2)
+LRRT_ATTENTION(f32_96x8, float, 96, 1)
 LRRT_ATTENTION(f32_128x8, float, 128, 1)
 LRRT_ATTENTION(bf16_64x8, __nv_bfloat16, 64, 1)
 LRRT_ATTENTION(bf16_64x16, __nv_bfloat16, 64, 2)
+LRRT_ATTENTION(bf16_96x8, __nv_bfloat16, 96, 1)
+LRRT_ATTENTION(bf16_96x16, __nv_bfloat16, 96, 2)
 LRRT_ATTENTION(bf16_128x8, __nv_bfloat16, 128, 1)
 LRRT_ATTENTION(bf16_128x16, __nv_bfloat16, 128, 2)
 LRRT_ATTENTION(bf16_256x8, __nv_bfloat16, 256, 1)
 LRRT_ATTENTION(f16_64x8, __half, 64, 1)
 LRRT_ATTENTION(f16_64x16, __half, 64, 2)
+LRRT_ATTENTION(f16_96x8, __half, 96, 1)
+LRRT_ATTENTION(f16_96x16, __half, 96, 2)
 LRRT_ATTENTION(f16_128x8, __half, 128, 1)
 LRRT_ATTENTION(f16_128x16, __half, 128, 2)
 LRRT_ATTENTION(f16_256x8, __half, 256, 1)

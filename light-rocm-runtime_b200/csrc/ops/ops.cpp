@@ -222,21 +222,34 @@ void rope_append(lro_context_t &context, const lro_rope_append_t &a) {
   // The widest vector that all rows and columns are made of: 16 bytes, 8 (for
   // 16-bit rows such as a half of 20 elements), or single elements. Measured with
   // 16384 tokens in bf16: 73, 109, 335 us.
+  // What is copied (values, and what is not turned) may take wider ones than the
+  // pairs: 6000 tokens of 56 heads over 8 of 80 elements in bf16, 40 of them turned,
+  // 40 us, and 54 with the pairs' vectors for all.
   const uint32_t half = a.rotary_dim / 2u, rest = dim - a.rotary_dim;
-  uint32_t width = 1;
+  const auto rows_and_cache_take = [&](size_t bytes) {
+    return rows_take(a.q, element, bytes) && rows_take(a.q_out, element, bytes) &&
+           rows_take(a.k, element, bytes) && rows_take(a.v, element, bytes) &&
+           cache_takes(a.cache, bytes);
+  };
+  uint32_t width = 1, copy_width = 1;
   for (const size_t bytes : {size_t{16}, size_t{8}}) {
     const uint32_t elements = static_cast<uint32_t>(bytes / element);
     const uint32_t angles = std::min(elements, 4u);
-    if (elements >= 4u && half % elements == 0 && rest % elements == 0 && dim % elements == 0 &&
-        rows_take(a.q, element, bytes) && rows_take(a.q_out, element, bytes) &&
-        rows_take(a.k, element, bytes) && rows_take(a.v, element, bytes) &&
-        cache_takes(a.cache, bytes) && multiple_of(a.cos_table, 4u * angles) &&
+    if (elements < 4u || rest % elements != 0 || dim % elements != 0 ||
+        !rows_and_cache_take(bytes)) {
+      continue;
+    }
+    copy_width = std::max(copy_width, elements);
+    if (half % elements == 0 && multiple_of(a.cos_table, 4u * angles) &&
         multiple_of(a.sin_table, 4u * angles)) {
       width = elements;
       break;
     }
   }
-  const uint32_t per_head = half / width + rest / width, per_value_head = dim / width;
+  if (width == 1) {
+    copy_width = 1;
+  }
+  const uint32_t per_head = half / width + rest / copy_width, per_value_head = dim / copy_width;
   const uint64_t per_token = (uint64_t{a.heads} + a.cache.kv_heads) * per_head;
   const uint64_t values_per_token = uint64_t{a.cache.kv_heads} * per_value_head;
   require((per_token + values_per_token) * a.tokens < (uint64_t{1} << 31),
@@ -262,7 +275,8 @@ void rope_append(lro_context_t &context, const lro_rope_append_t &a) {
   args.values_per_token = Divider::of(static_cast<uint32_t>(values_per_token));
   args.values_per_head = Divider::of(per_value_head);
   context.launch(std::string("ops_rope_") + (a.interleaved != 0 ? "pairs_" : "half_") +
-                     type_name(a.cache.type) + "_x" + std::to_string(width),
+                     type_name(a.cache.type) + "_x" + std::to_string(width) +
+                     (copy_width != width ? "x" + std::to_string(copy_width) : std::string()),
                  ceil_div(args.items, kRopeThreads) + ceil_div(args.value_items, kRopeThreads),
                  kRopeThreads, 0, args);
 }
@@ -287,7 +301,14 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
   require(cache_takes(a.cache, 16),
           "cache pointers and strides must be multiples of 16 bytes");
 
-  const uint32_t dim = a.cache.head_dim <= 64u ? 64u : a.cache.head_dim <= 128u ? 128u : 256u;
+  // The next of the kernels' widths: what lies past the head's elements are
+  // products of zeros. Heads of 96 in f32 (8 over 1, 6 sequences of about 90000
+  // keys) as 96 and as 128 elements: 98 and 115 us; of 80 in f16 (128 over 8, 8
+  // sequences of 3900): 35 and 38 us.
+  uint32_t dim = 256;
+  for (const uint32_t width : {128u, 96u, 64u}) {
+    dim = a.cache.head_dim <= width ? width : dim;
+  }
   const uint32_t group = a.heads / a.cache.kv_heads;
   // 16 query heads share a row that is read where their states fit the
   // registers; otherwise blocks of 8 read it one after another. Measured (128
@@ -319,7 +340,7 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
     tokens = std::min<uint64_t>(tokens, a.window);
   }
   const uint64_t rows = uint64_t{a.table.rows} * args.rows_per_sequence;
-  const uint32_t row_bytes = dim * static_cast<uint32_t>(element);
+  const uint32_t row_bytes = attention_row_bytes(dim, static_cast<uint32_t>(element));
   const uint32_t keys = attention_tile_keys(row_bytes);
   const uint64_t tiles = rows * (ceil_div(tokens, keys) + kAttentionRowCost);
   require(tiles < (uint64_t{1} << 31), "the table's tokens, times the kv heads, are too many");
