@@ -151,6 +151,41 @@ def test_attention_shapes(ops, torch, kind, dim, heads, kv_heads, page, layout):
     Attention(torch, kind, EDGES, heads, kv_heads, dim, page, layout).check(ops)
 
 
+@pytest.mark.parametrize("kind,dim,heads,kv_heads,page", [
+    ("f32", 72, 10, 2, 8), ("f32", 96, 24, 2, 16), ("f32", 88, 8, 1, 48), ("bf16", 72, 16, 1, 16),
+    ("bf16", 96, 14, 2, 8), ("f16", 88, 36, 3, 32), ("f16", 80, 3, 3, 1), ("bf16", 104, 12, 1, 24),
+])
+def test_attention_between_widths(ops, torch, kind, dim, heads, kv_heads, page):
+    """Heads of 65 to 127 elements, tiles of one page and of several."""
+    Attention(torch, kind, EDGES, heads, kv_heads, dim, page, seed=23).check(ops, window=300)
+
+
+@pytest.mark.parametrize("kind,dim", [("f32", 128), ("f32", 64), ("bf16", 64), ("f16", 256)])
+@pytest.mark.parametrize("page", [8, 16, 32])
+def test_attention_repeated_pages(ops, torch, kind, dim, page):
+    """A page that a sequence names twice, side by side: the same rows again."""
+    case = Attention(torch, kind, [100, 400, 64], 8, 2, dim, page, seed=25)
+    case.table[:, 1] = case.table[:, 0]
+    case.table[1, 3:6] = case.table[1, 2]
+    case.check(ops)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("spread", [0.01, 1.0, 12.0])
+def test_attention_wide_cap(ops, torch, kind, spread):
+    """Scores far below the cap and far above it. Beside the other errors a
+    capped score has that of 1 - 2 / (1 + e^2x): two units in the last place of
+    the exponential (2^-22), one of the reciprocal (2^-23), twice over: at most
+    2^-20 of the cap."""
+    cap = 50.0
+    case = Attention(torch, kind, [1, 40, 700, 2500], 16, 2, 96, 16, seed=27, spread=spread)
+    out, lse = ops.paged_attention(case.q, case.keys, case.values, case.table, case.n, softcap=cap)
+    want, want_lse, bound, lse_bound = case.expected(softcap=cap)
+    most = case.values[~case.values.isnan()].abs().max().double()
+    close(out, want, bound + 2 * 2.0 ** -20 * cap * most, "out")
+    close(lse, want_lse, lse_bound + 2.0 ** -20 * cap, "lse")
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("options", [
     dict(softcap=5.0), dict(window=1), dict(window=33), dict(window=100000), dict(scale=0.7),
@@ -371,6 +406,17 @@ def test_rope_append(ops, torch, kind, tokens, heads, kv_heads, dim, rotary, pag
     keys[place], limit[place], values[place] = want, bound, case["v"].double()
     close(case["keys"], keys, limit, "keys")
     assert torch.equal(case["values"].double(), values)
+
+
+@pytest.mark.parametrize("kind,heads,kv_heads,dim,rotary", [
+    ("bf16", 6, 2, 40, 40), ("f16", 4, 1, 72, 24), ("bf16", 3, 3, 56, 8), ("f16", 2, 1, 96, 88),
+    ("f16", 5, 1, 20, 8),
+])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rope_halves_of_odd_vectors(ops, torch, kind, heads, kv_heads, dim, rotary, interleaved):
+    """Halves of a multiple of four elements beside copies of a multiple of eight."""
+    test_rope_append(ops, torch, kind, 37, heads, kv_heads, dim, rotary, 12, interleaved)
+
 
 
 def test_rope_append_in_place_and_padding(ops, torch):
