@@ -89,12 +89,15 @@ struct RopeAppendArgs {
   Divider values_per_token, values_per_head;
 };
 
-// Shared memory of an attention block: a ring of tiles for each of its warps,
-// and a partial state for each. A tile is 16 keys and values, or 32 of the
-// short rows of 128 bytes: 8 KB, and 16 KB for rows of 512 bytes. Eight warps
+// Shared memory of an attention block: a ring of tiles for each of its units,
+// and a partial state for each. A unit is a warp, or two warps that share its
+// tiles, with eight heads each, where the states of 16 heads of a long row
+// would not fit one warp's registers. A tile is 16 keys and values, or 32 of the
+// short rows of 128 bytes: 8 KB, and 16 KB for rows of 512 bytes. Eight units
 // have three tiles each (two beside states of 16 heads); of the large tiles six
 // have two (four with three: 206 us instead of 179 for 64 sequences of up to 8192
-// keys, 4 heads of 128 in f32), four have three beside states of 256 elements.
+// keys, 4 heads of 128 in f32), four have three beside states of 256 elements, or
+// as teams (two beside 16 heads of 256).
 // Rows of 96 elements (for heads of 65 to 96) lie in the places of 128.
 LRRT_OPS_HD constexpr uint32_t attention_row_bytes(uint32_t dim, uint32_t element_bytes) {
   return (dim == 96u ? 128u : dim) * element_bytes;
@@ -105,12 +108,22 @@ LRRT_OPS_HD constexpr uint32_t attention_tile_bytes(uint32_t row_bytes) {
 LRRT_OPS_HD constexpr uint32_t attention_tile_keys(uint32_t row_bytes) {
   return attention_tile_bytes(row_bytes) / (2u * row_bytes);
 }
-LRRT_OPS_HD constexpr uint32_t attention_warps(uint32_t dim, uint32_t row_bytes) {
-  return row_bytes <= 256u ? 8u : dim <= 128u ? 6u : 4u;
+LRRT_OPS_HD constexpr uint32_t attention_team(uint32_t row_bytes, uint32_t heads) {
+  return heads > 8u && row_bytes > 256u ? 2u : 1u;
+}
+LRRT_OPS_HD constexpr uint32_t attention_units(uint32_t dim, uint32_t row_bytes,
+                                               uint32_t heads) {
+  return row_bytes <= 256u ? 8u : attention_team(row_bytes, heads) == 1u && dim <= 128u ? 6u : 4u;
+}
+LRRT_OPS_HD constexpr uint32_t attention_threads(uint32_t dim, uint32_t row_bytes,
+                                                 uint32_t heads) {
+  return 32u * attention_units(dim, row_bytes, heads) * attention_team(row_bytes, heads);
 }
 LRRT_OPS_HD constexpr uint32_t attention_stages(uint32_t dim, uint32_t row_bytes,
                                                 uint32_t heads) {
-  return heads > 8u || attention_warps(dim, row_bytes) == 6u ? 2u : 3u;
+  return attention_units(dim, row_bytes, heads) == 4u ? (dim > 128u && heads > 8u ? 2u : 3u)
+         : heads > 8u || row_bytes > 256u             ? 2u
+                                                      : 3u;
 }
 // One partial state: the weighted values (rows padded against bank conflicts),
 // the maxima and the sums of a block's heads.
@@ -119,7 +132,7 @@ LRRT_OPS_HD constexpr uint32_t attention_state_floats(uint32_t dim, uint32_t hea
 }
 LRRT_OPS_HD constexpr uint32_t attention_shared_bytes(uint32_t dim, uint32_t row_bytes,
                                                       uint32_t heads) {
-  return attention_warps(dim, row_bytes) *
+  return attention_units(dim, row_bytes, heads) *
              (attention_stages(dim, row_bytes, heads) * attention_tile_bytes(row_bytes) +
               4u * attention_state_floats(dim, heads)) +
          1024u;
@@ -128,7 +141,9 @@ static_assert(attention_shared_bytes(128, 256, 8) <= 232448u &&
                   attention_shared_bytes(128, 256, 16) <= 232448u &&
                   attention_shared_bytes(64, 256, 16) <= 232448u &&
                   attention_shared_bytes(128, 512, 8) <= 232448u &&
-                  attention_shared_bytes(256, 512, 8) <= 232448u,
+                  attention_shared_bytes(128, 512, 16) <= 232448u &&
+                  attention_shared_bytes(256, 512, 8) <= 232448u &&
+                  attention_shared_bytes(256, 512, 16) <= 232448u,
               "a block's shared memory");
 // Places that a block takes at least, so that a short row is not split into more
 // partial states than its tiles are worth. Measured (2000 bf16 keys of 8 heads of

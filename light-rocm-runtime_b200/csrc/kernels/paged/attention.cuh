@@ -5,10 +5,11 @@
 // l = l1 2^(m1 - m) + l2 2^(m2 - m), and the weighted values likewise.
 //
 // Bound by reading the cache once. What the layout does about that:
-//  - Every warp streams its own tiles (8 or 16 KB of keys and values) through
-//    shared-memory stages filled by cp.async, so a block keeps 128 to 192 KB in
-//    flight without a barrier between its warps. Rows are gathered through the
-//    page table, whose entries are read one tile ahead.
+//  - Every unit (a warp, or two with 8 of 16 heads each where the states of all
+//    would not fit a warp's registers) streams its own tiles (8 or 16 KB of keys
+//    and values) through shared-memory stages filled by cp.async, so a block keeps
+//    128 to 192 KB in flight without a barrier between its units. Rows are
+//    gathered through the page table, whose entries are read one tile ahead.
 //  - The query heads of one key-value head share each row that is read: scores
 //    are computed transposed, S^T = K Q^T, with 16 keys as the rows of the
 //    matrix product and 8 query heads as its columns, and so are the outputs,
@@ -18,9 +19,9 @@
 //    keep more than 16 bits; 32-bit operands into two TF32 parts (three
 //    products).
 //  - The tiles of all sequences and heads form one sequence that is cut into
-//    equal parts for the blocks, and each part into equal parts for the warps,
-//    whatever the lengths are. A row that lies within a warp's part is finished
-//    by that warp; the pieces of others are joined in shared memory, and where
+//    equal parts for the blocks, and each part into equal parts for the units,
+//    whatever the lengths are. A row that lies within a unit's part is finished
+//    by that unit; the pieces of others are joined in shared memory, and where
 //    a row lies in several blocks through the workspace by the last of them to
 //    arrive. Pieces are joined in their order, so that results do not depend on
 //    timing.
@@ -133,25 +134,30 @@ struct TileCursor {
   Span span;
 };
 
-template <typename T, int Dim, int HeadTiles> class PagedAttention {
+// Team: warps that share a unit's tiles, each with 8 * HeadTiles of the heads.
+template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
   static constexpr bool kWide = sizeof(T) == 4; // 32-bit elements
   static constexpr uint32_t kRowBytes = attention_row_bytes(Dim, sizeof(T)); // in a tile
-  static constexpr uint32_t kWarps = attention_warps(Dim, kRowBytes);
+  static constexpr uint32_t kHeads = 8u * HeadTiles * Team;
+  static constexpr uint32_t kUnits = attention_units(Dim, kRowBytes, kHeads);
+  static constexpr uint32_t kWarps = kUnits * Team;
   static constexpr uint32_t kKeys = attention_tile_keys(kRowBytes);
   static constexpr uint32_t kChunks = kRowBytes / 16u; // 16-byte chunks of a row
   static constexpr uint32_t kRowsPerPass = 32u / kChunks;
-  // Passes at once for tiles of several pages: all for the large tiles (8 keys a
-  // page, f32: 114 us, 125 with four), four for the small (short code: 130 us
-  // instead of 134 for 128 heads over 8 and one page).
-  static constexpr int kScatteredPasses = kRowBytes > 256u ? 16 : 4;
+  static constexpr uint32_t kPasses = kKeys / kRowsPerPass / Team; // of one warp
+  // Passes at once for tiles of several pages: all for large tiles (8 keys a
+  // page, f32: 114 us, 125 with four), four where that code is in the way of the
+  // rest (128 heads over 8, one page: 130 us instead of 134; teams of 16-bit
+  // elements 139 instead of 151).
+  static constexpr int kScatteredPasses = kRowBytes > 256u && (kWide || Team == 1) ? 16 : 4;
   static constexpr uint32_t kKeyTiles = kKeys / 16u;
-  static constexpr uint32_t kHeads = 8u * HeadTiles;
   static constexpr uint32_t kSteps = Dim * sizeof(T) / 32u; // of Q K^T (32 bytes of a row)
-  static constexpr uint32_t kStages = attention_stages(Dim, kRowBytes, 8u * HeadTiles);
+  static constexpr uint32_t kStages = attention_stages(Dim, kRowBytes, kHeads);
   static constexpr uint32_t kStageBytes = attention_tile_bytes(kRowBytes);
   static constexpr uint32_t kStateFloats = attention_state_floats(Dim, kHeads);
   static constexpr uint32_t kStateRow = Dim + 4u;           // floats of a head in a state
   static constexpr uint32_t kMaximaAt = kHeads * kStateRow; // then the sums
+  static_assert(Team == attention_team(kRowBytes, kHeads), "warps of a unit");
   static_assert(kChunks >= 8 && kChunks <= 32 && kKeys >= 16 && kKeys <= 32, "tile shape");
 
   // A row's chunk c is stored at c xor (row & 7): eight rows of a chunk column
@@ -160,7 +166,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     return row * kRowBytes + ((chunk ^ (row & 7u)) << 4u);
   }
 
-  struct Piece { // of a row that a warp leaves unfinished
+  struct Piece { // of a row that a unit leaves unfinished
     uint32_t row_begin, row_end; // the places of the row's tiles
     uint32_t sequence, row, present;
   };
@@ -170,17 +176,31 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
 
   const PagedAttentionArgs &args_;
   const uint32_t lane_ = threadIdx.x & 31u, warp_ = threadIdx.x >> 5u;
-  uint32_t ring_;          // this warp's stages
-  unsigned char *rings_;   // all warps'; at the end, the states of their last pieces
-  float *states_;          // shared: [kWarps] of the pieces that began before the warp's part
-  Piece *firsts_, *lasts_; // [kWarps] of either kind
+  const uint32_t unit_ = warp_ / Team, member_ = warp_ % Team;
+  uint32_t ring_;          // this unit's stages
+  unsigned char *rings_;   // all units'; at the end, the states of their last pieces
+  float *states_;          // shared: [kUnits] of the pieces that began before the unit's part
+  Piece *firsts_, *lasts_; // [kUnits] of either kind
   uint32_t *starts_;       // [kThreads] places before each thread's share; where states will be
-  uint32_t *seen_;         // [kStages] which keys of this warp's stages have a page
+  uint32_t *seen_;         // [kStages] which keys of this unit's stages have a page
   uint32_t *flags_;        // [2] whether the block joins its first, its last row
 
   uint32_t query_[HeadTiles][kSteps][kWide ? 4 : 2];
   float out_[HeadTiles][Dim / 16][4];
   float maximum_[HeadTiles][2], sum_[HeadTiles][2];
+
+  // The unit's warps.
+  __device__ __forceinline__ void unit_sync() const {
+    if constexpr (Team == 1) {
+      __syncwarp();
+    } else {
+      asm volatile("barrier.sync %0, %1;" ::"r"(1u + unit_), "n"(32 * Team) : "memory");
+    }
+  }
+  // A head of this warp's, among the block's.
+  __device__ __forceinline__ uint32_t head_at(int n) const {
+    return Team == 1 ? n * 8u : member_ * (8u * HeadTiles) + n * 8u;
+  }
 
   __device__ __forceinline__ uint32_t tiles_of(const Span &span) const {
     return (span.end - span.begin + kKeys - 1u) / kKeys;
@@ -239,7 +259,8 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     }
     const uint32_t page = present ? gather.page : 0u; // nothing is read there, zeros are written
     const Pages &k = args_.cache.keys, &v = args_.cache.values;
-    const uint32_t chunk = lane_ % kChunks, row_of_pass = lane_ / kChunks;
+    const uint32_t chunk = lane_ % kChunks;
+    const uint32_t row_of_pass = lane_ / kChunks + member_ * (kPasses * kRowsPerPass);
     const bool inside = chunk * (16u / sizeof(T)) < args_.head_dim;
     const uint32_t offset = inside ? chunk * 16u : 0u;
     const uint32_t wanted = inside ? seen >> row_of_pass : 0u;
@@ -257,7 +278,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
       const int64_t key_step = int64_t{k.token_stride} * (kRowsPerPass * sizeof(T));
       const int64_t value_step = int64_t{v.token_stride} * (kRowsPerPass * sizeof(T));
 #pragma unroll
-      for (uint32_t pass = 0; pass < kKeys / kRowsPerPass; ++pass) {
+      for (uint32_t pass = 0; pass < kPasses; ++pass) {
         const uint32_t at = to + swizzled(pass * kRowsPerPass + row_of_pass, chunk);
         const bool valid = (wanted >> pass * kRowsPerPass & 1u) != 0;
         if (chunk < Dim * sizeof(T) / 16u) {
@@ -271,7 +292,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
       const T *key = static_cast<const T *>(k.data) + k.offset(page, gather.row, gather.head);
       const T *value = static_cast<const T *>(v.data) + v.offset(page, gather.row, gather.head);
 #pragma unroll kScatteredPasses
-      for (uint32_t pass = 0; pass < kKeys / kRowsPerPass; ++pass) {
+      for (uint32_t pass = 0; pass < kPasses; ++pass) {
         const uint32_t row = pass * kRowsPerPass + row_of_pass;
         const uint64_t key_row =
             __shfl_sync(kAllLanes, reinterpret_cast<uint64_t>(key), row) + offset;
@@ -294,7 +315,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
                                                uint32_t heads) {
 #pragma unroll
     for (int n = 0; n < HeadTiles; ++n) {
-      const uint32_t head = n * 8u + lane_ / 4u;
+      const uint32_t head = head_at(n) + lane_ / 4u;
       const T *q = static_cast<const T *>(args_.q.data) +
                    args_.q.offset(sequence, first_head + min(head, heads - 1u));
       const uint32_t limit = head < heads ? args_.head_dim : 0u;
@@ -367,7 +388,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     for (int n = 0; n < HeadTiles; ++n) {
 #pragma unroll
       for (uint32_t i = 0; i < 2u; ++i) {
-        const uint32_t head = n * 8u + (lane_ & 3u) * 2u + i;
+        const uint32_t head = head_at(n) + (lane_ & 3u) * 2u + i;
         slope[n][i] =
             args_.slopes != nullptr && head < heads ? args_.slopes[first_head + head] : 0.0f;
       }
@@ -582,7 +603,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     for (int n = 0; n < HeadTiles; ++n) {
 #pragma unroll
       for (uint32_t i = 0; i < 2u; ++i) {
-        const uint32_t head = n * 8u + (lane_ & 3u) * 2u + i;
+        const uint32_t head = head_at(n) + (lane_ & 3u) * 2u + i;
         if (head >= heads) {
           continue;
         }
@@ -612,7 +633,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     for (int n = 0; n < HeadTiles; ++n) {
 #pragma unroll
       for (uint32_t i = 0; i < 4u; ++i) {
-        const uint32_t head = n * 8u + (lane_ & 3u) * 2u + (i & 1u);
+        const uint32_t head = head_at(n) + (lane_ & 3u) * 2u + (i & 1u);
 #pragma unroll
         for (uint32_t d = 0; d < Dim / 16u; ++d) {
           state[head * kStateRow + d * 16u + (i >> 1u) * 8u + lane_ / 4u] = out_[n][d][i];
@@ -662,20 +683,20 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     }
   }
 
-  // The pieces of one row that the block's warps left, from `warp` on: its
+  // The pieces of one row that the block's units left, from `unit` on: its
   // last one, or its first for a row from before the block. A row that other
   // blocks have a part of goes to `part`. By `threads` threads, this one the
   // `thread`th.
-  __device__ __forceinline__ void join_pieces(const Piece &piece, uint32_t warp, bool from_last,
+  __device__ __forceinline__ void join_pieces(const Piece &piece, uint32_t unit, bool from_last,
                                               float *part, uint32_t thread, uint32_t threads) {
     uint32_t count = 1;
-    while (warp + count < kWarps && firsts_[warp + count].present != 0 &&
-           firsts_[warp + count].row_begin == piece.row_begin) {
+    while (unit + count < kUnits && firsts_[unit + count].present != 0 &&
+           firsts_[unit + count].row_begin == piece.row_begin) {
       ++count;
     }
     const float *first_state =
-        from_last ? reinterpret_cast<const float *>(rings_ + warp * kStages * kStageBytes)
-                  : states_ + warp * kStateFloats;
+        from_last ? reinterpret_cast<const float *>(rings_ + unit * kStages * kStageBytes)
+                  : states_ + unit * kStateFloats;
     const HeadBlock heads = heads_of(piece.row);
 #pragma unroll 1
     for (uint32_t at = thread * 4u; at < heads.count * Dim; at += threads * 4u) {
@@ -685,7 +706,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
 #pragma unroll 2
       for (uint32_t i = 0; i < count; ++i) {
         joined.add_state(state, head, column);
-        state = states_ + (warp + i + 1u) * kStateFloats;
+        state = states_ + (unit + i + 1u) * kStateFloats;
       }
       if (part == nullptr) {
         finish(piece.sequence, heads.first + head, column, joined);
@@ -714,7 +735,7 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
   __device__ __forceinline__ void join_parts(const Piece &piece, uint32_t per_block) const {
     const uint32_t first = piece.row_begin / per_block, count = parts_of(piece, per_block);
     const HeadBlock heads = heads_of(piece.row);
-    constexpr uint32_t kRound = kWarps * kStages * kStageBytes / (4u * kStateFloats);
+    constexpr uint32_t kRound = kUnits * kStages * kStageBytes / (4u * kStateFloats);
     constexpr uint32_t kItems = kHeads * Dim / 4u;
     constexpr uint32_t kEach = (kItems + kThreads - 1u) / kThreads;
     const float *staged = reinterpret_cast<const float *>(rings_);
@@ -760,15 +781,15 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     }
   }
 
-  // Where warp w's tiles begin: equal parts, empty ones at the end alone.
-  static __device__ __forceinline__ uint32_t warp_part(uint32_t begin, uint32_t count,
-                                                       uint32_t w) {
-    return begin + count / kWarps * w + min(w, count % kWarps);
+  // Where unit u's tiles begin: equal parts, empty ones at the end alone.
+  static __device__ __forceinline__ uint32_t unit_part(uint32_t begin, uint32_t count,
+                                                       uint32_t u) {
+    return begin + count / kUnits * u + min(u, count % kUnits);
   }
 
   // Places: the tiles of all rows one after another, each row's followed by
   // kAttentionRowCost places that stand for the work a row takes besides its
-  // tiles. Blocks and warps take equal numbers of places.
+  // tiles. Blocks and units take equal numbers of places.
   __device__ __forceinline__ uint32_t places_of(uint32_t sequence) const {
     const uint32_t tiles = tiles_of(span_of(args_, sequence));
     return tiles == 0 ? 0u : (tiles + kAttentionRowCost) * args_.rows_per_sequence;
@@ -811,9 +832,9 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
     return start.before + (place - start.before + row - 1u) / row * row;
   }
 
-  // A warp's tiles, between the places begin and end, each loaded kStages - 1
+  // A unit's tiles, between the places begin and end, each loaded kStages - 1
   // steps ahead, and their page numbers two more.
-  __device__ __forceinline__ void run_warp(uint32_t begin, uint32_t end, const Start &start) {
+  __device__ __forceinline__ void run_unit(uint32_t begin, uint32_t end, const Start &start) {
     TileCursor at; // the tile to compute
     at.sequence = start.sequence;
     at.span = span_of(args_, at.sequence);
@@ -873,10 +894,10 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
         continue; // not all stages are under way yet
       }
       wait_copies<kStages - 1>();
-      __syncwarp();
+      unit_sync();
       compute(stage, at.span.begin + (tile - row_begin) * kKeys, at.span.end, heads.first,
               heads.count);
-      __syncwarp(); // the stage is filled again by the next issue
+      unit_sync(); // the stage is filled again by the next issue
       stage = stage + 1u == kStages ? 0u : stage + 1u;
       ++tile;
       if (tile != row_end && tile != end) {
@@ -886,17 +907,17 @@ template <typename T, int Dim, int HeadTiles> class PagedAttention {
       if (row_begin >= begin && row_end <= end) {
         finish_row(at.sequence, heads.first, heads.count);
       } else {
-        // A row from before the warp's part is its first; one that goes on
+        // A row from before the unit's part is its first; one that goes on
         // past it is its last, and nothing is left to load then.
         const bool is_first = row_begin < begin;
         if (!is_first) {
           wait_copies<0>();
-          __syncwarp();
+          unit_sync();
         }
-        save_state(is_first ? states_ + warp_ * kStateFloats
-                            : reinterpret_cast<float *>(rings_ + warp_ * kStages * kStageBytes));
-        if (lane_ == 0) {
-          (is_first ? firsts_ : lasts_)[warp_] = {row_begin, row_end, at.sequence, at.row, 1u};
+        save_state(is_first ? states_ + unit_ * kStateFloats
+                            : reinterpret_cast<float *>(rings_ + unit_ * kStages * kStageBytes));
+        if (lane_ == 0 && member_ == 0) {
+          (is_first ? firsts_ : lasts_)[unit_] = {row_begin, row_end, at.sequence, at.row, 1u};
         }
       }
       if (tile != row_end) {
@@ -919,17 +940,17 @@ public:
   __device__ __forceinline__ PagedAttention(const PagedAttentionArgs &args, unsigned char *shared)
       : args_(args) {
     rings_ = shared;
-    ring_ = shared_address(shared) + warp_ * kStages * kStageBytes;
-    unsigned char *at = shared + kWarps * kStages * kStageBytes;
+    ring_ = shared_address(shared) + unit_ * kStages * kStageBytes;
+    unsigned char *at = shared + kUnits * kStages * kStageBytes;
     states_ = reinterpret_cast<float *>(at);
-    at += 4u * kWarps * kStateFloats;
+    at += 4u * kUnits * kStateFloats;
     firsts_ = reinterpret_cast<Piece *>(at);
-    lasts_ = firsts_ + kWarps;
+    lasts_ = firsts_ + kUnits;
     starts_ = reinterpret_cast<uint32_t *>(states_);
-    seen_ = reinterpret_cast<uint32_t *>(lasts_ + kWarps) + warp_ * kStages;
-    flags_ = reinterpret_cast<uint32_t *>(lasts_ + kWarps) + kWarps * kStages;
-    static_assert(2u * sizeof(Piece) * kWarps + 4u * kStages * kWarps + 8u <= 1024u &&
-                      kThreads + 2u * kWarps <= kWarps * kStateFloats,
+    seen_ = reinterpret_cast<uint32_t *>(lasts_ + kUnits) + unit_ * kStages;
+    flags_ = reinterpret_cast<uint32_t *>(lasts_ + kUnits) + kUnits * kStages;
+    static_assert(2u * sizeof(Piece) * kUnits + 4u * kStages * kUnits + 8u <= 1024u &&
+                      kThreads + 2u * kWarps <= kUnits * kStateFloats,
                   "shared memory of the bookkeeping");
   }
 
@@ -954,8 +975,8 @@ public:
     if (lane_ == 31u) {
       warp_sums[warp_] = upto;
       warp_sums[kWarps + warp_] = most;
-      firsts_[warp_].present = 0;
-      lasts_[warp_].present = 0;
+      firsts_[unit_].present = 0;
+      lasts_[unit_].present = 0;
     }
     __syncthreads();
     uint32_t before = upto - mine, total = 0;
@@ -980,24 +1001,24 @@ public:
       end = row_boundary(end, total, share);
     }
     const uint32_t count = end - begin;
-    const uint32_t warp_begin = warp_part(begin, count, warp_);
-    const uint32_t warp_end = warp_part(begin, count, warp_ + 1u);
+    const uint32_t unit_begin = unit_part(begin, count, unit_);
+    const uint32_t unit_end = unit_part(begin, count, unit_ + 1u);
     Start start{0, 0};
-    if (warp_begin < warp_end) {
-      start = find(warp_begin, share);
+    if (unit_begin < unit_end) {
+      start = find(unit_begin, share);
     }
     __syncthreads(); // the starts lie where states will
-    if (warp_begin < warp_end) {
-      run_warp(warp_begin, warp_end, start);
+    if (unit_begin < unit_end) {
+      run_unit(unit_begin, unit_end, start);
     }
     __syncthreads();
-    // Rows from before the block (i = 0), then those that begin in warp i - 1:
+    // Rows from before the block (i = 0), then those that begin in unit i - 1:
     // one or two by all threads, more of them a warp each.
     const uint32_t present = __ballot_sync(
-        kAllLanes, lane_ <= kWarps &&
+        kAllLanes, lane_ <= kUnits &&
                        (lane_ == 0 ? firsts_[0] : lasts_[lane_ - 1u]).present != 0);
     const bool by_warp = __popc(present) > 2;
-    uint32_t go_on[2] = {kWarps + 1u, kWarps + 1u}; // those of other blocks too
+    uint32_t go_on[2] = {kUnits + 1u, kUnits + 1u}; // those of other blocks too
     uint32_t turn = 0;
 #pragma unroll 1
     for (uint32_t left = present; left != 0; left &= left - 1u, ++turn) {
@@ -1019,7 +1040,7 @@ public:
     if (threadIdx.x < 2u) {
       const uint32_t i = threadIdx.x == 0 ? go_on[0] : go_on[1];
       uint32_t last = 0;
-      if (i <= kWarps) {
+      if (i <= kUnits) {
         const Piece &piece = i == 0 ? firsts_[0] : lasts_[i - 1u];
         uint32_t *arrivals =
             args_.arrivals + size_t{piece.sequence} * args_.rows_per_sequence + piece.row;

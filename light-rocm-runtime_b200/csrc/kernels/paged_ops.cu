@@ -32,32 +32,37 @@ LRRT_ROPE(f16_x4x8, __half, 4, 8)
 LRRT_ROPE(f16_x4, __half, 4, 4)
 LRRT_ROPE(f16_x1, __half, 1, 1)
 
-#define LRRT_ATTENTION(name, type, dim, head_tiles)                                               \
-  extern "C" __global__ void __launch_bounds__(PagedAttention<type, dim, head_tiles>::kThreads, 1) \
+#define LRRT_ATTENTION(name, type, dim, head_tiles, team)                                         \
+  extern "C" __global__ void                                                                      \
+      __launch_bounds__(PagedAttention<type, dim, head_tiles, team>::kThreads, 1)                 \
       ops_attention_##name(const __grid_constant__ PagedAttentionArgs args) {                     \
     extern __shared__ __align__(128) unsigned char shared[];                                      \
     wait_for_previous_launch();                                                                   \
-    PagedAttention<type, dim, head_tiles>(args, shared).run();                                    \
+    PagedAttention<type, dim, head_tiles, team>(args, shared).run();                              \
   }
 
-LRRT_ATTENTION(f32_64x8, float, 64, 1)
-LRRT_ATTENTION(f32_64x16, float, 64, 2)
-LRRT_ATTENTION(f32_96x8, float, 96, 1)
-LRRT_ATTENTION(f32_128x8, float, 128, 1)
-LRRT_ATTENTION(bf16_64x8, __nv_bfloat16, 64, 1)
-LRRT_ATTENTION(bf16_64x16, __nv_bfloat16, 64, 2)
-LRRT_ATTENTION(bf16_96x8, __nv_bfloat16, 96, 1)
-LRRT_ATTENTION(bf16_96x16, __nv_bfloat16, 96, 2)
-LRRT_ATTENTION(bf16_128x8, __nv_bfloat16, 128, 1)
-LRRT_ATTENTION(bf16_128x16, __nv_bfloat16, 128, 2)
-LRRT_ATTENTION(bf16_256x8, __nv_bfloat16, 256, 1)
-LRRT_ATTENTION(f16_64x8, __half, 64, 1)
-LRRT_ATTENTION(f16_64x16, __half, 64, 2)
-LRRT_ATTENTION(f16_96x8, __half, 96, 1)
-LRRT_ATTENTION(f16_96x16, __half, 96, 2)
-LRRT_ATTENTION(f16_128x8, __half, 128, 1)
-LRRT_ATTENTION(f16_128x16, __half, 128, 2)
-LRRT_ATTENTION(f16_256x8, __half, 256, 1)
+LRRT_ATTENTION(f32_64x8, float, 64, 1, 1)
+LRRT_ATTENTION(f32_64x16, float, 64, 2, 1)
+LRRT_ATTENTION(f32_96x8, float, 96, 1, 1)
+LRRT_ATTENTION(f32_96x16, float, 96, 1, 2)
+LRRT_ATTENTION(f32_128x8, float, 128, 1, 1)
+LRRT_ATTENTION(f32_128x16, float, 128, 1, 2)
+LRRT_ATTENTION(bf16_64x8, __nv_bfloat16, 64, 1, 1)
+LRRT_ATTENTION(bf16_64x16, __nv_bfloat16, 64, 2, 1)
+LRRT_ATTENTION(bf16_96x8, __nv_bfloat16, 96, 1, 1)
+LRRT_ATTENTION(bf16_96x16, __nv_bfloat16, 96, 2, 1)
+LRRT_ATTENTION(bf16_128x8, __nv_bfloat16, 128, 1, 1)
+LRRT_ATTENTION(bf16_128x16, __nv_bfloat16, 128, 2, 1)
+LRRT_ATTENTION(bf16_256x8, __nv_bfloat16, 256, 1, 1)
+LRRT_ATTENTION(bf16_256x16, __nv_bfloat16, 256, 1, 2)
+LRRT_ATTENTION(f16_64x8, __half, 64, 1, 1)
+LRRT_ATTENTION(f16_64x16, __half, 64, 2, 1)
+LRRT_ATTENTION(f16_96x8, __half, 96, 1, 1)
+LRRT_ATTENTION(f16_96x16, __half, 96, 2, 1)
+LRRT_ATTENTION(f16_128x8, __half, 128, 1, 1)
+LRRT_ATTENTION(f16_128x16, __half, 128, 2, 1)
+LRRT_ATTENTION(f16_256x8, __half, 256, 1, 1)
+LRRT_ATTENTION(f16_256x16, __half, 256, 1, 2)
 
 #define LRRT_PLAN(name, args_type)                                                                \
   extern "C" __global__ void __cluster_dims__(kPlanBlocks, 1, 1) __launch_bounds__(kPlanThreads)  \

@@ -310,12 +310,12 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
     dim = a.cache.head_dim <= width ? width : dim;
   }
   const uint32_t group = a.heads / a.cache.kv_heads;
-  // 16 query heads share a row that is read where their states fit the
-  // registers; otherwise blocks of 8 read it one after another. Measured (128
-  // heads over 8, 64 ragged sequences): 16 heads and twice 8, bf16 of 128 elements
-  // 138 and 223 us, of 64 97 and 158 us, f32 of 64 181 and 216 us.
-  const bool sixteen = group > 8u && dim <= (a.cache.type == LRO_F32 ? 64u : 128u);
-  const uint32_t heads = sixteen ? 16u : 8u;
+  // Up to 16 query heads share a row that is read; blocks of them read it one
+  // after another. Measured (64 ragged sequences of up to 8192 keys), blocks of 16
+  // heads and of 8: bf16, 128 heads over 8, of 128 elements 128 and 226 us, of 64 86
+  // and 156 us; 64 over 4 of 256 139 and 239 us; f32, 128 over 8 of 64 178 and 226 us,
+  // 48 over 4 of 128 249 and 318 us.
+  const uint32_t heads = group > 8u ? 16u : 8u;
   PagedAttentionArgs args{};
   args.q = rows_of(a.q);
   args.out = rows_of(a.out);
@@ -352,7 +352,7 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
   args.arrivals = static_cast<uint32_t *>(context.counters->data());
   context.launch(std::string("ops_attention_") + type_name(a.cache.type) + "_" +
                      std::to_string(dim) + "x" + std::to_string(heads),
-                 grid, 32u * attention_warps(dim, row_bytes),
+                 grid, attention_threads(dim, row_bytes, heads),
                  attention_shared_bytes(dim, row_bytes, heads), args);
 }
 
