@@ -292,7 +292,7 @@ struct BeamArgs {
   uint64_t *part_keys;    // [rows][parts][count]
   Pair *part_sums;        // [rows][parts] maximum, sum of exponentials
   uint64_t *row_keys;     // [rows][count]
-  float *row_log_sums;    // [rows]
+  double *row_log_sums;   // [rows]
   uint32_t *row_arrivals; // [rows], zero between launches
   uint32_t *group_arrivals; // [groups], likewise
 };
