@@ -16,8 +16,8 @@
 //    O^T = V^T P^T. One query row per head leaves nothing to fill the 128 rows
 //    of a tcgen05 tile from the query side; these shapes (m16n8) waste none.
 //    16-bit weights are split into two 16-bit parts, so that the probabilities
-//    keep more than 16 bits; 32-bit operands into two TF32 parts (three
-//    products).
+//    keep 16 bits (in f16 down to 2^-39 of a row's largest); 32-bit operands into
+//    two TF32 parts (three products).
 //  - The tiles of all sequences and heads form one sequence that is cut into
 //    equal parts for the blocks, and each part into equal parts for the units,
 //    whatever the lengths are. A row that lies within a unit's part is finished
@@ -115,6 +115,14 @@ __device__ __forceinline__ void split_16(float x, float y, uint32_t &high, uint3
   memcpy(&b, &ly, 2);
   low = uint32_t{a} | uint32_t{b} << 16;
 }
+
+// Weights are taken 2^kWeightBits times as large, and their sums with them, so that
+// f16, which ends at 2^-24, holds those far below a row's largest one: its two
+// parts then end at 2^-39 of it. Without, a key 17 below another in its score
+// weighed nothing in the products and 4e-8 in the sum. (The largest is 2^15, and
+// f16 goes on to 2^16.) bf16 has the exponents of 32 bits.
+template <typename T> constexpr float kWeightBits = 0.0f;
+template <> constexpr float kWeightBits<__half> = 15.0f;
 
 // The keys of a sequence that a step sees.
 struct Span {
@@ -499,7 +507,7 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
       for (uint32_t m = 0; m < kKeyTiles; ++m) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = exp2_fast(score[n][m][i] - base[i % 2]);
+          const float p = exp2_fast(score[n][m][i] - (base[i % 2] - kWeightBits<T>));
           score[n][m][i] = p;
           sum_[n][i % 2] += p;
         }
@@ -592,7 +600,7 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
                                             float sum) const {
     if (args_.lse != nullptr) {
       args_.lse[uint64_t{sequence} * args_.heads + head] =
-          top == -INFINITY ? -INFINITY : (top + log2f(sum)) * kLn2;
+          top == -INFINITY ? -INFINITY : (top + (log2f(sum) - kWeightBits<T>)) * kLn2;
     }
   }
 
