@@ -596,11 +596,13 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
     }
   }
 
+  // A sum of 0 is that of a row that sees no token: the largest weight is
+  // 2^kWeightBits. Where all scores are NaN the maximum is -infinity too.
   __device__ __forceinline__ void write_lse(uint32_t sequence, uint32_t head, float top,
                                             float sum) const {
     if (args_.lse != nullptr) {
       args_.lse[uint64_t{sequence} * args_.heads + head] =
-          top == -INFINITY ? -INFINITY : (top + (log2f(sum) - kWeightBits<T>)) * kLn2;
+          sum == 0.0f ? -INFINITY : (top + (log2f(sum) - kWeightBits<T>)) * kLn2;
     }
   }
 
@@ -616,7 +618,7 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
           continue;
         }
         const float top = maximum_[n][i];
-        const float inverse = top == -INFINITY ? 0.0f : 1.0f / sum_[n][i];
+        const float inverse = sum_[n][i] == 0.0f ? 0.0f : 1.0f / sum_[n][i];
         T *out = static_cast<T *>(args_.out.data) +
                  args_.out.offset(sequence, first_head + head);
 #pragma unroll
@@ -677,7 +679,7 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
 
   __device__ __forceinline__ void finish(uint32_t sequence, uint32_t head, uint32_t column,
                                          const Joined &joined) const {
-    const float inverse = joined.top == -INFINITY ? 0.0f : 1.0f / joined.sum;
+    const float inverse = joined.sum == 0.0f ? 0.0f : 1.0f / joined.sum;
     T *out = static_cast<T *>(args_.out.data) + args_.out.offset(sequence, head);
     const float x[4] = {joined.x.x, joined.x.y, joined.x.z, joined.x.w};
 #pragma unroll

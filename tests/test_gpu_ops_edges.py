@@ -1,5 +1,7 @@
 """The paged-cache operators where numbers are at the ends of their ranges.
 Bounds are derived as in test_gpu_ops.py."""
+import math
+
 import pytest
 
 from test_gpu_ops import FLOAT, LEAST, ROUND, Attention, close, ops, torch  # noqa: F401
@@ -65,3 +67,19 @@ def test_attention_below_a_dominating_key(ops, torch, kind, first, n, gap, equal
     want_lse = torch.logsumexp(x, 0).expand(1, 8)
     sums = (2.0 ** -18 * (1 - 1 / total) + (2 * tiles + 156) * FLOAT).cpu()
     close(lse, want_lse, sums + 4 * FLOAT * want_lse.abs().cpu(), "lse")
+
+
+# --- infinities and NaN -----------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lengths", [[5, 40], [700, 3], [20000, 16]])
+def test_attention_nan_rows(ops, torch, kind, lengths):
+    """A NaN in a query: outputs and log-sums of its head are NaN, and no others."""
+    case = Attention(torch, kind, lengths, 8, 2, 64, 16, seed=33)
+    case.q[0, 2, 5] = math.nan
+    out, lse = ops.paged_attention(case.q, case.keys, case.values, case.table, case.n)
+    nan = torch.zeros(2, 8, dtype=torch.bool, device="cuda")
+    nan[0, 2] = True
+    assert torch.equal(lse.isnan(), nan)
+    assert torch.equal(out.isnan().all(-1), nan) and torch.equal(out.isnan().any(-1), nan)
+    assert lse[~nan].isfinite().all()
