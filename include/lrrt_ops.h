@@ -119,9 +119,11 @@ LRRT_API lr_status_t lro_rope_append(lro_context_t *context, const lro_rope_appe
  *   s_j = x_j - slopes[h] * (lengths[b] - 1 - j)   (slopes may be NULL)
  *   out = sum_j exp(s_j) v_j / sum_j exp(s_j),  lse = log sum_j exp(s_j)
  * over the tokens j that have a page and, with window > 0, are among the last
- * `window`. A row that sees no token has out = 0 and lse = -infinity; lengths
- * are clamped to [0, columns * page_size]. Sums are held in 32 bits; 32-bit
- * products are three TF32 products (about 2^-21 per product).
+ * `window`. A row that sees no token, or none with a score above -infinity, has
+ * out = 0 and lse = -infinity; lengths are clamped to [0, columns * page_size].
+ * An infinite value makes its column infinite (NaN with both signs); a NaN, or
+ * a score of infinity, leaves NaN in out and lse. Sums are held in 32 bits;
+ * 32-bit products are three TF32 products (about 2^-21 per product).
  * head_dim: a multiple of 8, at most 256 (128 in 32 bits). Cache pointers and
  * strides: multiples of 16 bytes.
  */

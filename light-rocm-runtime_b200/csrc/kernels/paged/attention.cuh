@@ -101,19 +101,45 @@ __device__ __forceinline__ void split_tf32(uint32_t bits, uint32_t &high, uint32
   low = __float_as_uint(__uint_as_float(bits) - __uint_as_float(high)) & 0xffffe000u;
 }
 
-// Two floats as a pair of 16-bit numbers, and what the rounding left over as
-// another.
-template <typename T>
-__device__ __forceinline__ void split_16(float x, float y, uint32_t &high, uint32_t &low) {
-  const T hx = from_float<T>(x), hy = from_float<T>(y);
-  const T lx = from_float<T>(x - to_float(hx)), ly = from_float<T>(y - to_float(hy));
-  uint16_t a, b;
-  memcpy(&a, &hx, 2);
-  memcpy(&b, &hy, 2);
-  high = uint32_t{a} | uint32_t{b} << 16;
-  memcpy(&a, &lx, 2);
-  memcpy(&b, &ly, 2);
-  low = uint32_t{a} | uint32_t{b} << 16;
+// Weights and values are split so that infinite values go through: both parts of
+// a weight are positive, so that an infinity times them is that infinity (0, and a
+// negative rest, would make a NaN of it), and the second part of an infinite value
+// is finite. Weights and values are cut off after their first part, not rounded:
+// the rest has their sign, and NaN stays NaN.
+
+// A weight as two TF32 numbers; 2^-126 is nothing beside any sum.
+__device__ __forceinline__ void split_weight_tf32(uint32_t bits, uint32_t &high, uint32_t &low) {
+  high = bits & 0xffffe000u;
+  low = __float_as_uint(fmaxf(__uint_as_float(bits) - __uint_as_float(high), 0x1p-126f));
+}
+
+// A value: the rest is below 2^-10 of the largest number. That of an infinity is
+// a NaN before the minimum.
+__device__ __forceinline__ void split_value_tf32(uint32_t bits, uint32_t &high, uint32_t &low) {
+  high = bits & 0xffffe000u;
+  const float rest = __uint_as_float(bits) - __uint_as_float(high);
+  low = __float_as_uint(fminf(rest, 0x1p118f)) & 0xffffe000u;
+}
+
+// Two weights as a pair of 16-bit numbers, and what they leave over as another. In
+// f16 the least number, 2^-39 of the largest weight, stands for a first part of 0.
+__device__ __forceinline__ void split_weights(float x, float y, uint32_t &high, uint32_t &low,
+                                              __nv_bfloat16) {
+  high = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+  const __nv_bfloat162 rest = __floats2bfloat162_rn(x - __uint_as_float(high << 16),
+                                                    y - __uint_as_float(high & 0xffff0000u));
+  memcpy(&low, &rest, 4);
+  asm("max.bf16x2 %0, %0, %1;" : "+r"(low) : "r"(0x00800080u)); // 2^-126
+}
+__device__ __forceinline__ void split_weights(float x, float y, uint32_t &high, uint32_t &low,
+                                              __half) {
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(high) : "f"(y), "f"(x));
+  __half2 first;
+  memcpy(&first, &high, 4);
+  const __half2 rest = __floats2half2_rn(x - __low2float(first), y - __high2float(first));
+  memcpy(&low, &rest, 4);
+  asm("max.f16x2 %0, %0, %1;" : "+r"(low) : "r"(0x00010001u));
+  asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(high) : "r"(0x00010001u));
 }
 
 // Weights are taken 2^kWeightBits times as large, and their sums with them, so that
@@ -385,10 +411,29 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
     }
   }
 
+  // The product of a query and a key of the tile at `keys`, by 32-bit arithmetic.
+  static __device__ __noinline__ float whole_score(const PagedAttentionArgs &args, uint32_t keys,
+                                                   uint32_t key, uint32_t sequence,
+                                                   uint32_t first_head, uint32_t head,
+                                                   uint32_t heads) {
+    float sum = 0.0f;
+    if (head < heads) {
+      const T *q =
+          static_cast<const T *>(args.q.data) + args.q.offset(sequence, first_head + head);
+#pragma unroll 1
+      for (uint32_t d = 0; d < args.head_dim; ++d) {
+        const uint32_t word = load_shared(keys + swizzled(key, d / 4u) + (d & 3u) * 4u);
+        sum = fmaf(to_float(q[d]), __uint_as_float(word), sum);
+      }
+    }
+    return sum;
+  }
+
   // One tile of keys: scores, weights and weighted values. Score registers
   // i of a 16 x 8 tile: key lane / 4 + (i / 2) * 8, head (lane % 4) * 2 + i % 2.
   __device__ __forceinline__ void compute(uint32_t stage, uint32_t first_key, uint32_t end,
-                                          uint32_t first_head, uint32_t heads) {
+                                          uint32_t sequence, uint32_t first_head,
+                                          uint32_t heads) {
     const uint32_t keys = ring_ + stage * kStageBytes;
     const uint32_t values = keys + kStageBytes / 2u;
     float slope[HeadTiles][2]; // under way before the products; 0 without a bias
@@ -442,6 +487,36 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
             multiply(score[n][m], a, query_[n][k][0], query_[n][k][1], T());
           }
         }
+      }
+    }
+    if constexpr (kWide) {
+      // The two parts of an infinity, or of a number that rounds to one, make a
+      // NaN: such scores are summed anew from the numbers themselves.
+      bool finite = true;
+#pragma unroll
+      for (int n = 0; n < HeadTiles; ++n) {
+#pragma unroll
+        for (uint32_t m = 0; m < kKeyTiles; ++m) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            finite = finite && fabsf(score[n][m][i]) < INFINITY;
+          }
+        }
+      }
+      if (!__all_sync(kAllLanes, finite)) {
+#pragma unroll
+        for (int n = 0; n < HeadTiles; ++n) {
+#pragma unroll
+          for (uint32_t m = 0; m < kKeyTiles; ++m) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              score[n][m][i] = whole_score(args_, keys, m * 16u + (i / 2) * 8u + lane_ / 4u,
+                                           sequence, first_head,
+                                           head_at(n) + (lane_ & 3u) * 2u + i % 2, heads);
+            }
+          }
+        }
+        __syncwarp();
       }
     }
     const uint32_t seen = seen_[stage];
@@ -527,8 +602,8 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
             const uint32_t y = __float_as_uint(score[n][m][2u * part + 1u]);
             const uint32_t lows = transpose_matrix(__byte_perm(x, y, 0x5410));
             const uint32_t highs = transpose_matrix(__byte_perm(x, y, 0x7632));
-            split_tf32(__byte_perm(lows, highs, 0x5410), weight[n][0], weight[n][2]);
-            split_tf32(__byte_perm(lows, highs, 0x7632), weight[n][1], weight[n][3]);
+            split_weight_tf32(__byte_perm(lows, highs, 0x5410), weight[n][0], weight[n][2]);
+            split_weight_tf32(__byte_perm(lows, highs, 0x7632), weight[n][1], weight[n][3]);
           }
           // Column k of the product is key 2 k, and column k + 4 key 2 k + 1.
           const uint32_t key = m * 16u + part * 8u + (lane_ & 3u) * 2u;
@@ -540,7 +615,7 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
               const uint32_t column = d * 16u + (i & 1u) * 8u + lane_ / 4u;
               const uint32_t word = load_shared(values + swizzled(key + (i >> 1u), column / 4u) +
                                                 (column & 3u) * 4u);
-              split_tf32(word, high[i], low[i]);
+              split_value_tf32(word, high[i], low[i]);
             }
 #pragma unroll
             for (int n = 0; n < HeadTiles; ++n) {
@@ -562,7 +637,7 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
 #pragma unroll
           for (uint32_t part = 0; part < 2u; ++part) {
             uint32_t high, low;
-            split_16<T>(score[n][m][2u * part], score[n][m][2u * part + 1u], high, low);
+            split_weights(score[n][m][2u * part], score[n][m][2u * part + 1u], high, low, T());
             weight[n][part] = transpose_matrix(high);
             weight[n][2u + part] = transpose_matrix(low);
           }
@@ -905,8 +980,8 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
       }
       wait_copies<kStages - 1>();
       unit_sync();
-      compute(stage, at.span.begin + (tile - row_begin) * kKeys, at.span.end, heads.first,
-              heads.count);
+      compute(stage, at.span.begin + (tile - row_begin) * kKeys, at.span.end, at.sequence,
+              heads.first, heads.count);
       unit_sync(); // the stage is filled again by the next issue
       stage = stage + 1u == kStages ? 0u : stage + 1u;
       ++tile;

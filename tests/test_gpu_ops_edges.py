@@ -9,6 +9,14 @@ from test_gpu_ops import FLOAT, LEAST, ROUND, Attention, close, ops, torch  # no
 pytestmark = pytest.mark.gpu
 
 
+def same(actual, want, bound, what=""):
+    """close(), and NaN in the same places."""
+    actual, want = actual.double().cpu(), want.double().cpu()
+    assert (actual.isnan() == want.isnan()).all(), f"{what}: NaN elsewhere"
+    clean = lambda x: x.nan_to_num(nan=0.0, posinf=math.inf, neginf=-math.inf)  # noqa: E731
+    close(clean(actual), clean(want), bound.nan_to_num(0.0, 0.0, 0.0), what)
+
+
 # --- weights far below the largest ------------------------------------------------
 
 def dominated(torch, kind, n, gap, first, equal, dim=64):
@@ -83,3 +91,91 @@ def test_attention_nan_rows(ops, torch, kind, lengths):
     assert torch.equal(lse.isnan(), nan)
     assert torch.equal(out.isnan().all(-1), nan) and torch.equal(out.isnan().any(-1), nan)
     assert lse[~nan].isfinite().all()
+
+
+@pytest.mark.parametrize("kind,dim,heads,kv_heads", [
+    ("f32", 64, 14, 2), ("f32", 128, 24, 2), ("f32", 128, 8, 2), ("f32", 96, 3, 3),
+    ("bf16", 128, 32, 8), ("bf16", 64, 24, 2), ("bf16", 256, 20, 1), ("f16", 128, 16, 2),
+    ("f16", 256, 17, 1), ("f16", 80, 4, 4),
+])
+@pytest.mark.parametrize("lengths", [[1, 37], [300, 1000], [20000, 0]])
+def test_attention_infinite_values(ops, torch, kind, dim, heads, kv_heads, lengths):
+    """An infinite value makes its column infinite, of both signs NaN, a NaN
+    NaN; every other column is as it would be."""
+    case = Attention(torch, kind, lengths, heads, kv_heads, dim, 16, seed=35)
+    bound = case.expected()[2]  # with the finite values: the largest one is the same
+
+    def put(row, j, head, column, value):
+        case.values[int(case.table[row, j // 16]), j % 16, head, column] = value
+
+    for row, n in enumerate(lengths):
+        if n:
+            put(row, n // 2, 0, 1, math.inf)
+            put(row, n - 1, 0, 2, -math.inf)
+            put(row, 0, kv_heads - 1, 5, math.inf)
+            put(row, n // 3, kv_heads - 1, 7, math.nan)
+        if n > 30:
+            put(row, n - 9, 0, 3, math.inf)
+            put(row, 4, 0, 3, -math.inf)
+    out, lse = ops.paged_attention(case.q, case.keys, case.values, case.table, case.n)
+    want, want_lse, _, lse_bound = case.expected()
+    same(out, want, bound, "out")
+    same(lse, want_lse, lse_bound, "lse")
+    if lengths[0] > 30:
+        assert (out[0, :heads // kv_heads, 1] == math.inf).all()
+        assert (out[0, :heads // kv_heads, 2] == -math.inf).all()
+        assert out[0, :heads // kv_heads, 3].isnan().all()
+
+
+@pytest.mark.parametrize("kind,dim,heads,kv_heads", [
+    ("f32", 64, 14, 2), ("f32", 128, 24, 2), ("f32", 128, 8, 2), ("f32", 96, 3, 3),
+    ("bf16", 128, 8, 2), ("bf16", 256, 20, 1), ("f16", 64, 24, 2),
+])
+@pytest.mark.parametrize("lengths", [[3, 37], [300, 1000], [20000, 50]])
+def test_attention_infinite_keys(ops, torch, kind, dim, heads, kv_heads, lengths):
+    """A key whose score is -infinity weighs nothing, one of infinity leaves NaN."""
+    case = Attention(torch, kind, lengths, heads, kv_heads, dim, 16, seed=37)
+    case.q[:, :, 3] = case.q[:, :, 3].abs() + 0.5
+    _, _, bound, lse_bound = case.expected()  # an infinity has no error of its own
+
+    def put(row, j, heads, value):
+        case.keys[int(case.table[row, j // 16]), j % 16, heads, 3] = value
+
+    for j in {0, lengths[0] // 2}:
+        put(0, j, slice(None), -math.inf)
+    put(1, lengths[1] - 1, 0, math.inf)
+    want, want_lse, _, _ = case.expected()
+    group = heads // kv_heads
+    assert want[0].isfinite().all() and want[1, :group].isnan().all()
+    out, lse = ops.paged_attention(case.q, case.keys, case.values, case.table, case.n)
+    same(out, want, bound + 1.01 * ROUND[kind] * want.abs(), "out")
+    want_lse[1, :group] = math.nan  # infinity - infinity, as the weights are
+    same(lse, want_lse, lse_bound + 4 * FLOAT * want_lse.abs(), "lse")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+def test_attention_nothing_weighs(ops, torch, kind):
+    """Every score is -infinity: as a row that sees no token."""
+    case = Attention(torch, kind, [1, 20, 5000], 8, 2, 64, 16, seed=39)
+    case.q[:, :, 0] = 1
+    case.keys[..., 0] = -math.inf
+    out, lse = ops.paged_attention(case.q, case.keys, case.values, case.table, case.n)
+    assert (out == 0).all() and (lse == -math.inf).all()
+
+
+def test_attention_largest_numbers(ops, torch):
+    """Keys and values next to the largest of 32 bits: what rounds to an infinity
+    on its way is still the number that it is."""
+    most = torch.finfo(torch.float32).max
+    lengths = [1, 33, 900]
+    case = Attention(torch, "f32", lengths, 8, 2, 64, 16, seed=41)
+    case.keys[..., 2] = most
+    case.q[..., 2] = 2.0 ** -122
+    want, want_lse, bound, lse_bound = case.expected()
+    case.values[..., 1] = most
+    out, lse = ops.paged_attention(case.q, case.keys, case.values, case.table, case.n)
+    others = [i for i in range(64) if i != 1]
+    close(out[..., others], want[..., others], bound[..., others], "out")
+    close(lse, want_lse, lse_bound, "lse")
+    # One key: its value, split in two (2^-20). More of them may leave 32 bits.
+    assert ((out[0, :, 1].double() / most - 1).abs() <= 2.0 ** -19).all()
