@@ -85,9 +85,23 @@ __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], 
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// c = a b for TF32.
+// c = a b.
 __device__ __forceinline__ void multiply_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
-                                               uint32_t b1) {
+                                               uint32_t b1, __nv_bfloat16) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+               "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void multiply_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1, __half) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+               "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void multiply_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1, float) {
   asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, "
                "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
                : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
@@ -473,7 +487,7 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
 #pragma unroll
           for (int n = 0; n < HeadTiles; ++n) {
             float part[4];
-            multiply_first(part, low, query_[n][k][0], query_[n][k][1]);
+            multiply_first(part, low, query_[n][k][0], query_[n][k][1], T());
             multiply(part, high, query_[n][k][2], query_[n][k][3], T());
             multiply(part, high, query_[n][k][0], query_[n][k][1], T());
 #pragma unroll
@@ -589,10 +603,13 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
       }
     }
     // O^T += V^T P^T. The weights are transposed in registers: a lane then
-    // holds head lane / 4 and keys (lane % 4) * 2, + 1 of eight.
+    // holds head lane / 4 and keys (lane % 4) * 2, + 1 of eight. A tile's products
+    // are summed by themselves, the tiles in rounded 32 bits: the tensor cores' sums
+    // drop the bits below the last of the sum so far, and a row of 100000 keys
+    // that one warp summed there came out 5e-4 too small.
+    if constexpr (kWide) {
 #pragma unroll
-    for (uint32_t m = 0; m < kKeyTiles; ++m) {
-      if constexpr (kWide) {
+      for (uint32_t m = 0; m < kKeyTiles; ++m) {
 #pragma unroll
         for (uint32_t part = 0; part < 2u; ++part) { // eight keys a product
           uint32_t weight[HeadTiles][4]; // high, high, low, low of the two keys
@@ -620,7 +637,7 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
 #pragma unroll
             for (int n = 0; n < HeadTiles; ++n) {
               float part[4];
-              multiply_first(part, low, weight[n][0], weight[n][1]);
+              multiply_first(part, low, weight[n][0], weight[n][1], T());
               multiply(part, high, weight[n][2], weight[n][3], T());
               multiply(part, high, weight[n][0], weight[n][1], T());
 #pragma unroll
@@ -630,27 +647,46 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
             }
           }
         }
-      } else {
-        uint32_t weight[HeadTiles][4]; // high of keys 0-7 and 8-15, low of them
+      }
+    } else {
+      uint32_t weight[kKeyTiles][HeadTiles][4]; // high of keys 0-7 and 8-15, low of them
+#pragma unroll
+      for (uint32_t m = 0; m < kKeyTiles; ++m) {
 #pragma unroll
         for (int n = 0; n < HeadTiles; ++n) {
 #pragma unroll
           for (uint32_t part = 0; part < 2u; ++part) {
             uint32_t high, low;
             split_weights(score[n][m][2u * part], score[n][m][2u * part + 1u], high, low, T());
-            weight[n][part] = transpose_matrix(high);
-            weight[n][2u + part] = transpose_matrix(low);
+            weight[m][n][part] = transpose_matrix(high);
+            weight[m][n][2u + part] = transpose_matrix(low);
           }
         }
-        const uint32_t row = m * 16u + (lane_ >> 4u) * 8u + (lane_ & 7u);
+      }
+      const uint32_t row = (lane_ >> 4u) * 8u + (lane_ & 7u);
 #pragma unroll
-        for (int d = 0; d < Dim / 16; ++d) {
+      for (int d = 0; d < Dim / 16; ++d) {
+        float part[HeadTiles][4];
+#pragma unroll
+        for (uint32_t m = 0; m < kKeyTiles; ++m) {
           uint32_t a[4];
-          load_matrices_transposed(a, values + swizzled(row, 2u * d + (lane_ >> 3u & 1u)));
+          load_matrices_transposed(
+              a, values + swizzled(m * 16u + row, 2u * d + (lane_ >> 3u & 1u)));
 #pragma unroll
           for (int n = 0; n < HeadTiles; ++n) {
-            multiply(out_[n][d], a, weight[n][2], weight[n][3], T());
-            multiply(out_[n][d], a, weight[n][0], weight[n][1], T());
+            if (m == 0) {
+              multiply_first(part[n], a, weight[m][n][2], weight[m][n][3], T());
+            } else {
+              multiply(part[n], a, weight[m][n][2], weight[m][n][3], T());
+            }
+            multiply(part[n], a, weight[m][n][0], weight[m][n][1], T());
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < HeadTiles; ++n) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            out_[n][d][i] += part[n][i];
           }
         }
       }

@@ -4,7 +4,7 @@ import math
 
 import pytest
 
-from test_gpu_ops import FLOAT, LEAST, ROUND, Attention, close, ops, torch  # noqa: F401
+from test_gpu_ops import FLOAT, LEAST, ROUND, Attention, close, dtype_of, ops, torch  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +179,28 @@ def test_attention_largest_numbers(ops, torch):
     close(lse, want_lse, lse_bound, "lse")
     # One key: its value, split in two (2^-20). More of them may leave 32 bits.
     assert ((out[0, :, 1].double() / most - 1).abs() <= 2.0 ** -19).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("dim,heads", [(64, 8), (128, 16)])
+def test_attention_long_sums(ops, torch, kind, dim, heads):
+    """Rows of 100000 keys, so many that a warp has nearly all of one, with the
+    same value at each key: the output is that value. Rounded to nearest, the
+    tiles' sums are off by a random walk of 6250 roundings of 2^-24 (3e-6), less
+    than half a unit in the last place of 16 bits; rounded one way, by 4e-4."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(43)
+    n, batch, page = 100000, 1200, 64
+    pages = -(-n // page)
+    dtype = dtype_of(torch, kind)
+    keys = (torch.randn(pages, page, 1, dim, generator=g, device="cuda") * 0.3).to(dtype)
+    value = (1 + torch.arange(dim, device="cuda") / 128).to(dtype)
+    values = value.expand(pages, page, 1, dim).contiguous()
+    q = torch.randn(batch, heads, dim, generator=g, device="cuda").to(dtype)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").expand(batch, -1)
+    lengths = torch.full((batch,), n, dtype=torch.int32, device="cuda")
+    out, _ = ops.paged_attention(q, keys, values, table, lengths)
+    if kind == "f32":
+        close(out, value.expand_as(out), 2.0 ** -16 * value.expand_as(out), "out")
+    else:
+        assert torch.equal(out, value.expand_as(out))
