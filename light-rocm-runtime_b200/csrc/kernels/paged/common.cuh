@@ -188,13 +188,6 @@ __device__ __forceinline__ uint32_t arrive(uint32_t *counter) {
   return before;
 }
 
-// 1 / x to a unit or so in the last place; 0 for infinity.
-__device__ __forceinline__ float reciprocal_fast(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

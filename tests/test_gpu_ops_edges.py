@@ -204,3 +204,14 @@ def test_attention_long_sums(ops, torch, kind, dim, heads):
         close(out, value.expand_as(out), 2.0 ** -16 * value.expand_as(out), "out")
     else:
         assert torch.equal(out, value.expand_as(out))
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("softcap", [0.5, 50.0, 1.0e3, 1.0e4, 1.0e6])
+@pytest.mark.parametrize("spread", [0.01, 1.0, 12.0])
+def test_attention_caps(ops, torch, kind, softcap, spread):
+    """Caps below the scores and far above them. A capped score has the relative
+    error of two products and of tanhf, below 2^-21,
+    which the bound of every score (2^-19 of its products' sizes) holds."""
+    case = Attention(torch, kind, [1, 40, 700, 2500], 16, 2, 96, 16, seed=45, spread=spread)
+    case.check(ops, softcap=softcap)
