@@ -290,9 +290,10 @@ struct BeamArgs {
   uint32_t parts, part_elements; // of a row; elements a multiple of 8
   int32_t end_token;
   uint64_t *part_keys;    // [rows][parts][count]
-  Pair *part_sums;        // [rows][parts] maximum, sum of exponentials
+  Pair *part_sums;        // [rows][parts] maximum, sum of exponentials above it
   uint64_t *row_keys;     // [rows][count]
-  double *row_log_sums;   // [rows]
+  float *row_tops;        // [rows] maximum
+  double *row_log_sums;   // [rows] logarithm of the sum above it
   uint32_t *row_arrivals; // [rows], zero between launches
   uint32_t *group_arrivals; // [groups], likewise
 };

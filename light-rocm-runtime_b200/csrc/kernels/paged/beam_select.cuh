@@ -234,11 +234,19 @@ __device__ __noinline__ uint64_t prune_share(uint64_t *share, uint32_t held, uin
   return bound;
 }
 
-// Maximum (times log2 e) and sum of a set of elements, and of two sets.
+// e^(x - base), 1 where they are equal at any size: rows may be masked throughout
+// with a type's lowest value, whose product with log2 e leaves 32 bits. (x log2 e -
+// base log2 e in one instruction took 22.7 us where this takes 23.6, 256 rows of 151936
+// in bf16; it lost all of a sum above 1e10, and 8e-4 of its logarithm at 6e4.)
+__device__ __forceinline__ float exp_above(float x, float base) {
+  return exp2_fast((x - base) * kLog2E);
+}
+
+// Maximum and sum of a set of elements, and of two sets.
 __device__ __forceinline__ float2 join_sums(float2 a, float2 b) {
   const float top = fmaxf(a.x, b.x);
   const float base = top == -INFINITY ? 0.0f : top;
-  return make_float2(top, a.y * exp2_fast(a.x - base) + b.y * exp2_fast(b.x - base));
+  return make_float2(top, a.y * exp_above(a.x, base) + b.y * exp_above(b.x, base));
 }
 __device__ __forceinline__ float2 join_lanes(float2 mine) {
 #pragma unroll
@@ -249,18 +257,18 @@ __device__ __forceinline__ float2 join_lanes(float2 mine) {
   return mine;
 }
 
-// The logarithm of a sum of exponentials, whose maximum is in base 2. It goes into
-// all scores of its row, so it is kept in 64 bits and scores are rounded once:
-// without the sum's exponent log2f is below 1, and its last place as small.
-// (In 32 bits scores were 1.1e-7 off, relative to their sizes; now 0.4e-7.)
-__device__ __forceinline__ double log_of(float2 all) {
-  float whole = 0.0f, rest = all.y;
+// The logarithm of a row's sum, relative to its maximum. It goes into all scores of
+// the row, so it is kept in 64 bits and scores are rounded once: without the sum's
+// exponent log2f is below 1, and its last place as small. (In 32 bits scores were
+// 1.1e-7 off, relative to their sizes; now 0.4e-7.)
+__device__ __forceinline__ double log_of(float sum) {
+  float whole = 0.0f, rest = sum;
   if (rest >= 1.0f && rest < INFINITY) {
     const uint32_t bits = __float_as_uint(rest);
     whole = static_cast<float>(static_cast<int32_t>(bits >> 23) - 127);
     rest = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u);
   }
-  return (double{all.x} + (double{whole} + double{log2f(rest)})) * 0.69314718055994531;
+  return (double{whole} + double{log2f(rest)}) * 0.69314718055994531;
 }
 
 // Whether this block is the last of `blocks` to get here; its reads then see
@@ -294,9 +302,10 @@ __device__ __forceinline__ void rank_beams(const BeamArgs &args, uint32_t group,
     if (args.finished == nullptr || args.finished[row] == 0) {
       const uint64_t key = __ldcg(args.row_keys + uint64_t{row} * args.count + rank);
       const float logit = value_of(static_cast<uint32_t>(key >> 32));
+      const double above = double{logit} - __ldcg(args.row_tops + row); // exact, or nearly
       score = key == kNoKey ? -INFINITY
                             : static_cast<float>(double{score} +
-                                                 (logit - __ldcg(args.row_log_sums + row)));
+                                                 (above - __ldcg(args.row_log_sums + row)));
     } else if (rank != 0) {
       score = -INFINITY;
     }
@@ -397,12 +406,12 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
       const float most = fmaxf(W::largest(larger_word), -INFINITY); // NaN counts as -infinity
       shared.noted[number][threadIdx.x] = most;
       largest = fmaxf(largest, most);
-      const float now = fmaxf(top, most * kLog2E);
+      const float now = fmaxf(top, most);
       const float base = now == -INFINITY ? 0.0f : now;
       float each[4] = {}; // four sums at a time
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        each[i % 4] += exp2_fast(fmaf(W::value(from[i / kPerWord], i % kPerWord), kLog2E, -base));
+        each[i % 4] += exp_above(W::value(from[i / kPerWord], i % kPerWord), base);
       }
       float terms = (each[0] + each[1]) + (each[2] + each[3]);
       if (terms != terms) { // there is a NaN
@@ -411,10 +420,10 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
         for (int i = 0; i < kEach; ++i) {
           const uint32_t index = index_of(round, i);
           const float y = index < whole ? to_float(logits[index]) : -INFINITY;
-          terms += y == y ? exp2_fast(fmaf(y, kLog2E, -base)) : 0.0f;
+          terms += y == y ? exp_above(y, base) : 0.0f;
         }
       }
-      sum = sum * exp2_fast(top - base) + terms;
+      sum = sum * exp_above(top, base) + terms;
       top = now;
     };
     // Each thread has its own elements copied, so that rounds need no barrier;
@@ -455,7 +464,7 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
       odd = to_float(logits[odd_index(threadIdx.x)]);
       odd = odd == odd ? odd : -INFINITY;
       largest = fmaxf(largest, odd);
-      const float2 joined = join_sums(make_float2(top, sum), make_float2(odd * kLog2E, 1.0f));
+      const float2 joined = join_sums(make_float2(top, sum), make_float2(odd, 1.0f));
       top = joined.x;
       sum = joined.y;
     }
@@ -573,7 +582,8 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
       if (args.parts != 1u) {
         args.part_sums[slot] = {all.x, all.y};
       } else {
-        args.row_log_sums[row] = log_of(all);
+        args.row_tops[row] = all.x;
+        args.row_log_sums[row] = log_of(all.y);
       }
     }
   }
@@ -596,7 +606,8 @@ __device__ __forceinline__ void beam_select(const BeamArgs &args) {
             join_lanes(join_sums(lane < args.parts ? __ldcg(sums + lane) : none,
                                  lane + 32u < args.parts ? __ldcg(sums + lane + 32u) : none));
         if (lane == 0) {
-          args.row_log_sums[row] = log_of(all);
+          args.row_tops[row] = all.x;
+          args.row_log_sums[row] = log_of(all.y);
         }
       }
       rank_pool(total, args.count, shared);

@@ -564,8 +564,9 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
   parts = ceil_div(a.vocab, part_elements);
   const size_t sums_at = aligned(8u * rows * parts * a.count),
                row_keys_at = sums_at + aligned(8u * rows * parts),
-               log_sums_at = row_keys_at + aligned(8u * rows * a.count);
-  context.reserve(log_sums_at + aligned(8u * rows));
+               log_sums_at = row_keys_at + aligned(8u * rows * a.count),
+               tops_at = log_sums_at + aligned(8u * rows);
+  context.reserve(tops_at + aligned(4u * rows));
   context.reserve_counters(rows + a.groups);
   auto *scratch = static_cast<unsigned char *>(context.scratch->data());
   auto *counters = static_cast<uint32_t *>(context.counters->data());
@@ -588,6 +589,7 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
   args.part_keys = reinterpret_cast<uint64_t *>(scratch);
   args.part_sums = reinterpret_cast<Pair *>(scratch + sums_at);
   args.row_keys = reinterpret_cast<uint64_t *>(scratch + row_keys_at);
+  args.row_tops = reinterpret_cast<float *>(scratch + tops_at);
   args.row_log_sums = reinterpret_cast<double *>(scratch + log_sums_at);
   args.row_arrivals = counters;
   args.group_arrivals = counters + rows;

@@ -215,3 +215,40 @@ def test_attention_caps(ops, torch, kind, softcap, spread):
     which the bound of every score (2^-19 of its products' sizes) holds."""
     case = Attention(torch, kind, [1, 40, 700, 2500], 16, 2, 96, 16, seed=45, spread=spread)
     case.check(ops, softcap=softcap)
+
+
+# --- rows of masked logits --------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("mask", ["lowest", -1.0e10, -1.0e30, 1.0e10, "largest", -60000.0])
+@pytest.mark.parametrize("vocab", [70, 5000, 151936])
+def test_beam_select_masked_rows(ops, torch, kind, mask, vocab):
+    """A row of one value throughout, as masks of a type's lowest value leave it, is
+    uniform: its best are the lowest tokens, at -log vocab. Beside it a row where
+    the mask leaves three tokens, and one that it leaves as it is.
+
+    Scores are off by the roundings of 32 bits and by the sum's (2^-18, as in
+    test_gpu_ops.py); a beam's logits are exact in each type."""
+    dtype = dtype_of(torch, kind)
+    info = torch.finfo(dtype)
+    value = {"lowest": info.min, "largest": info.max}.get(mask, mask)
+    value = min(max(value, info.min), info.max)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(47)
+    rows = torch.randn(3, vocab, generator=g, device="cuda").mul_(48).round_().div_(16)
+    rows[0] = value
+    if value < 0:
+        rows[1, 3:] = value
+    logits = rows.to(dtype)
+    assert (logits[0] == logits[0, 0]).all() and logits.isfinite().all()
+    scores = torch.tensor([-3.0, -30.0, -60.0], device="cuda")
+    got = ops.beam_select(logits[None], scores[None], 16)
+    x = logits.double()
+    above = x - x.amax(-1, keepdim=True)
+    score = scores.double()[:, None] + above - above.exp().sum(-1, keepdim=True).log()
+    order = score.flatten().sort(descending=True, stable=True)
+    close(got[0][0], order.values[:16], torch.tensor(2.0 ** -18 + 4 * 64 * FLOAT), "scores")
+    alone = ops.beam_select(logits[None, :1], scores[None, :1], 16)
+    assert alone[2].tolist() == [list(range(16))] and alone[1].tolist() == [[0] * 16]
+    close(alone[0][0], torch.full((16,), -3.0 - math.log(vocab)),
+          torch.tensor(2.0 ** -18 + 4 * 64 * FLOAT), "scores")
