@@ -136,16 +136,17 @@ __device__ __noinline__ void rank_pool(uint32_t total, uint32_t count, BeamShare
     // One, two or four threads for a key, each counting among as many others.
     const uint32_t shift = total <= kBeamThreads / 4u ? 2u : total <= kBeamThreads / 2u ? 1u : 0u;
     const uint32_t parts = 1u << shift, at = thread >> shift;
-    if (at < (total + 7u & ~7u)) { // whole warps
+    const uint32_t of_warp = 32u >> shift; // keys
+    if (thread / 32u * of_warp < total) {  // whole warps, the last one's surplus without keys
       const uint64_t key = at < total ? shared.pool[at] : kNoKey;
       uint32_t rank = 0;
 #pragma unroll 8
       for (uint32_t j = thread & (parts - 1u); j < total; j += parts) {
         rank += shared.pool[j] > key ? 1u : 0u;
       }
-      const unsigned lanes = __activemask();
-      rank += shift > 0u ? __shfl_xor_sync(lanes, rank, 1) : 0u;
-      rank += shift > 1u ? __shfl_xor_sync(lanes, rank, 2) : 0u;
+      // The lanes' loops differ in length, so all of the warp's are waited for.
+      rank += shift > 0u ? __shfl_xor_sync(kAllLanes, rank, 1) : 0u;
+      rank += shift > 1u ? __shfl_xor_sync(kAllLanes, rank, 2) : 0u;
       if (at < total && rank < count) {
         shared.best[rank] = key_or_none(key);
       }

@@ -2,9 +2,11 @@
 Bounds are derived as in test_gpu_ops.py."""
 import math
 
+import numpy as np
 import pytest
 
-from test_gpu_ops import FLOAT, LEAST, ROUND, Attention, close, dtype_of, ops, torch  # noqa: F401
+from test_gpu_ops import (FLOAT, LEAST, ROUND, Attention, beam_case, beam_check, close,  # noqa: F401
+                          dtype_of, ops, torch)
 
 pytestmark = pytest.mark.gpu
 
@@ -252,3 +254,16 @@ def test_beam_select_masked_rows(ops, torch, kind, mask, vocab):
     assert alone[2].tolist() == [list(range(16))] and alone[1].tolist() == [[0] * 16]
     close(alone[0][0], torch.full((16,), -3.0 - math.log(vocab)),
           torch.tensor(2.0 ** -18 + 4 * 64 * FLOAT), "scores")
+
+
+# --- every number of candidates ---------------------------------------------------
+
+@pytest.mark.parametrize("beams", [1, 2, 3, 5, 7, 8, 13, 16])
+def test_beam_select_any_number_of_candidates(ops, torch, beams):
+    """Few candidates are ranked by one, two or four threads each, whatever remains
+    of the last warp: all numbers of them up to 17 beams' worth."""
+    rng = np.random.default_rng(beams)
+    for count in range(1, 18):
+        logits, scores, finished = beam_case(rng, 3, beams, 200)
+        beam_check(ops, torch, "f32", logits, scores, count, finished, end_token=1)
+        beam_check(ops, torch, "bf16", logits, scores, count)
