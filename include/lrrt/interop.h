@@ -20,6 +20,14 @@ extern "C" {
  */
 LRRT_API lr_status_t lr_queue_wrap_stream(lr_device_t device, void *stream, lr_queue_t **queue);
 
+/*
+ * Whether work given to the queue (NULL: the device's default queue) is being
+ * captured in a CUDA graph: nothing may be allocated or freed for it then. 1
+ * too where the queue is the legacy default stream and another is captured.
+ */
+LRRT_API lr_status_t lr_queue_is_capturing(lr_device_t device, lr_queue_t *queue,
+                                           uint32_t *capturing);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,15 +66,20 @@ typedef struct lro_table_t {
 /*
  * A context: the operators' module (paged_ops.cubin), the queue they run on
  * (NULL: the device's default queue; it must outlive the context) and a
- * workspace. The workspace grows when a call needs more of it, which drains
- * the device: before capturing calls in a CUDA graph make one of the same
- * sizes, or reserve.
+ * workspace, with counters that blocks meet at. Both grow when a call needs more
+ * of them; what they outgrow stays until the context is destroyed, so that CUDA
+ * graphs captured before can be replayed after. While its queue is captured a
+ * call that would have to grow them fails: make a call of the same sizes before,
+ * or reserve. An attention needs a counter for each sequence and key-value head,
+ * and each 16 of its query heads; a selection one for each beam and each
+ * group; 16384 are there.
  */
 LRRT_API lr_status_t lro_context_create(lr_device_t device, lr_queue_t *queue,
                                         const void *module_image, size_t module_image_size,
                                         lro_context_t **context);
 LRRT_API lr_status_t lro_context_destroy(lro_context_t *context);
 LRRT_API lr_status_t lro_context_reserve(lro_context_t *context, size_t workspace_bytes);
+LRRT_API lr_status_t lro_context_reserve_counters(lro_context_t *context, uint64_t counters);
 
 /*
  * cos/sin tables [positions][rotary_dim / 2] (host arrays), computed in 64 bits

@@ -3,6 +3,7 @@
 // device code is paged_ops.cubin (csrc/kernels/paged_ops.cu).
 #include "lrrt_ops.h"
 
+#include "lrrt/interop.h"
 #include "lrrt/lrrt.hpp"
 #include "lrrt/ops/kernels.hpp"
 
@@ -13,6 +14,8 @@
 #include <stdexcept>
 #include <string>
 #include <unordered_map>
+#include <utility>
+#include <vector>
 
 namespace {
 
@@ -143,22 +146,40 @@ struct lro_context_t {
     reserve_counters(16384);
   }
 
-  // Work on the queue may still use the buffers: freeing one drains the device.
   void reserve(size_t bytes) {
     if (!scratch || scratch->size() < bytes) {
-      scratch.reset();
-      scratch.emplace(device, aligned(bytes));
+      grow(scratch, bytes, false);
     }
   }
 
   // Counters are zero between calls: the kernels put them back.
   void reserve_counters(size_t count) {
     if (!counters || counters->size() < 4u * count) {
-      counters.reset();
-      counters.emplace(device, aligned(4u * count));
-      launch("ops_zero", 64, 256, 0,
-             ZeroArgs{static_cast<uint32_t *>(counters->data()), counters->size() / 4u});
+      grow(counters, 4u * count, true);
     }
+  }
+
+  // A larger buffer takes the place of one, which stays: work on the queue and
+  // captured graphs may still use it. Sizes double at least, so that all that is
+  // kept is no larger than what is in use.
+  void grow(std::optional<lrrt::DeviceBuffer> &buffer, size_t bytes, bool zero) {
+    uint32_t capturing = 0;
+    lrrt::check(lr_queue_is_capturing(device.get(), queue, &capturing), "lr_queue_is_capturing");
+    if (capturing != 0) {
+      throw std::runtime_error("the workspace is too small for this call, and cannot grow while "
+                               "its stream is captured: reserve it before");
+    }
+    outgrown.reserve(outgrown.size() + 1u);
+    lrrt::DeviceBuffer larger(device,
+                              aligned(std::max(bytes, buffer ? 2u * buffer->size() : size_t{0})));
+    if (zero) {
+      launch("ops_zero", 64, 256, 0,
+             ZeroArgs{static_cast<uint32_t *>(larger.data()), larger.size() / 4u});
+    }
+    if (buffer) {
+      outgrown.push_back(std::move(*buffer));
+    }
+    buffer.emplace(std::move(larger));
   }
 
   lr_kernel_t *kernel(const std::string &name) {
@@ -192,6 +213,7 @@ struct lro_context_t {
   lrrt::Module module;
   std::unordered_map<std::string, lr_kernel_t *> kernels;
   std::optional<lrrt::DeviceBuffer> scratch, counters;
+  std::vector<lrrt::DeviceBuffer> outgrown;
   uint32_t sms = 0;
 };
 
@@ -623,6 +645,14 @@ LRRT_API lr_status_t lro_context_reserve(lro_context_t *context, size_t workspac
   return guarded("lro_context_reserve", [&] {
     require(context != nullptr, "context is null");
     context->reserve(workspace_bytes);
+  });
+}
+
+LRRT_API lr_status_t lro_context_reserve_counters(lro_context_t *context, uint64_t counters) {
+  return guarded("lro_context_reserve_counters", [&] {
+    require(context != nullptr, "context is null");
+    require(counters < (uint64_t{1} << 40), "too many counters");
+    context->reserve_counters(counters);
   });
 }
 

@@ -27,6 +27,7 @@ namespace lrrt_b200 {
   X(cuStreamCreate)                                                            \
   X(cuStreamDestroy)                                                           \
   X(cuStreamSynchronize)                                                       \
+  X(cuStreamIsCapturing)                                                       \
   X(cuStreamWaitEvent)                                                         \
   X(cuEventCreate)                                                             \
   X(cuEventDestroy)                                                            \

@@ -684,6 +684,30 @@ LRRT_API lr_status_t lr_queue_wrap_stream(lr_device_t device, void *stream,
   return LR_SUCCESS;
 }
 
+LRRT_API lr_status_t lr_queue_is_capturing(lr_device_t device, lr_queue_t *queue,
+                                           uint32_t *capturing) {
+  Lock lock(g_mutex);
+  if (!g_initialized) {
+    return LR_ERROR_NOT_INITIALIZED;
+  }
+  DeviceState *state = open_device_state(device.index);
+  if (state == nullptr || capturing == nullptr ||
+      (queue != nullptr && (g_queues.count(queue) == 0 || queue->device != device.index))) {
+    return LR_ERROR_INVALID_ARGUMENT;
+  }
+  LR_TRY(make_current(*state));
+  CUstreamCaptureStatus status = CU_STREAM_CAPTURE_STATUS_NONE;
+  const CUresult result = g_driver.cuStreamIsCapturing_(
+      queue != nullptr ? queue->stream : state->stream, &status);
+  if (result == CUDA_ERROR_STREAM_CAPTURE_IMPLICIT) {
+    *capturing = 1;
+    return LR_SUCCESS;
+  }
+  LR_TRY(cu(result, "cuStreamIsCapturing"));
+  *capturing = status != CU_STREAM_CAPTURE_STATUS_NONE ? 1u : 0u;
+  return LR_SUCCESS;
+}
+
 LRRT_API lr_status_t lr_queue_destroy(lr_queue_t *queue) {
   Lock lock(g_mutex);
   if (!g_initialized) {

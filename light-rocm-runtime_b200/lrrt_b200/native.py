@@ -226,6 +226,7 @@ RUNTIME_FUNCTIONS = {
     "lr_queue_native_handle": (u32, [Device, vp, P(vp)]),
     "lr_last_error_detail": (u32, [C.c_char_p, sz]),
     "lr_queue_wrap_stream": (u32, [Device, vp, P(vp)]),
+    "lr_queue_is_capturing": (u32, [Device, vp, P(u32)]),
 }
 
 DRIVER_FUNCTIONS = {
@@ -278,6 +279,7 @@ OPS_FUNCTIONS = {
     "lro_context_create": (u32, [Device, vp, vp, sz, P(vp)]),
     "lro_context_destroy": (u32, [vp]),
     "lro_context_reserve": (u32, [vp, sz]),
+    "lro_context_reserve_counters": (u32, [vp, u64]),
     "lro_rope_tables": (u32, [u32, u32, f64, f64, f64, f64, f64, P(f32), P(f32)]),
     "lro_rope_append": (u32, [vp, P(RopeAppend)]),
     "lro_paged_attention": (u32, [vp, P(PagedAttention)]),

@@ -90,10 +90,14 @@ class Ops:
     def __exit__(self, *exc):
         self.close()
 
-    def reserve(self, workspace_bytes: int) -> None:
-        """Workspace for later calls, so that none of them has to grow it."""
+    def reserve(self, workspace_bytes: int, counters: int = 0) -> None:
+        """Workspace and counters for later calls, so that none of them has to
+        grow them, which a call that is captured cannot (lro_context_create
+        says what calls need)."""
         N.check(N.operators().lro_context_reserve(self.handle, workspace_bytes),
                 "lro_context_reserve")
+        N.check(N.operators().lro_context_reserve_counters(self.handle, counters),
+                "lro_context_reserve_counters")
 
     # ---- operators -----------------------------------------------------------
     def rope_append(self, q, k, v, keys, values, table, sequences, positions, cos, sin,
