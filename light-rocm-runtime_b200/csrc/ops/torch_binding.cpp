@@ -57,18 +57,19 @@ const Ops &ops_of(PyObject *capsule) {
   return *ops;
 }
 
-// One call of the library, other Python threads running meanwhile.
-template <typename Arguments>
-void call_library(lr_status_t (*function)(lro_context_t *, const Arguments *), const Ops &ops,
-                  const Arguments &arguments, const char *operation) {
-  lr_status_t status;
-  Py_BEGIN_ALLOW_THREADS;
-  status = function(ops.context, &arguments);
-  Py_END_ALLOW_THREADS;
+void check(lr_status_t status, const char *operation) {
   if (status != LR_SUCCESS) {
     Py_XDECREF(PyObject_CallFunction(g_fail, "is", static_cast<int>(status), operation));
     throw Raised{};
   }
+}
+
+// One call of the library. It enqueues and returns, and the interpreter's lock is
+// kept meanwhile: a context serves one thread at a time.
+template <typename Arguments>
+void call_library(lr_status_t (*function)(lro_context_t *, const Arguments *), const Ops &ops,
+                  const Arguments &arguments, const char *operation) {
+  check(function(ops.context, &arguments), operation);
 }
 
 // ---- tensors ------------------------------------------------------------------
@@ -462,6 +463,30 @@ PyObject *open_ops(PyObject *, PyObject *arguments) {
   }
 }
 
+// reserve(ops, workspace_bytes, counters), on whatever stream.
+PyObject *reserve_ops(PyObject *, PyObject *arguments) {
+  PyObject *capsule = nullptr;
+  unsigned long long bytes = 0, counters = 0;
+  if (!PyArg_ParseTuple(arguments, "OKK", &capsule, &bytes, &counters)) {
+    return nullptr;
+  }
+  const auto *ops = static_cast<const Ops *>(PyCapsule_GetPointer(capsule, kOpsCapsule));
+  if (ops == nullptr) {
+    return nullptr;
+  }
+  if (ops->context == nullptr) {
+    PyErr_SetString(PyExc_ValueError, "these operators are closed");
+    return nullptr;
+  }
+  try {
+    check(lro_context_reserve(ops->context, bytes), "lro_context_reserve");
+    check(lro_context_reserve_counters(ops->context, counters), "lro_context_reserve_counters");
+  } catch (const Raised &) {
+    return nullptr;
+  }
+  Py_RETURN_NONE;
+}
+
 // close(ops): its context is about to be destroyed.
 PyObject *close_ops(PyObject *, PyObject *capsule) {
   auto *ops = static_cast<Ops *>(PyCapsule_GetPointer(capsule, kOpsCapsule));
@@ -477,6 +502,7 @@ PyObject *close_ops(PyObject *, PyObject *capsule) {
    METH_FASTCALL, nullptr}
 
 PyMethodDef g_methods[] = {{"open", open_ops, METH_VARARGS, nullptr},
+                           {"reserve", reserve_ops, METH_VARARGS, nullptr},
                            {"close", close_ops, METH_O, nullptr},
                            LRRT_ENTRY(rope_append, 13),
                            LRRT_ENTRY(paged_attention, 11),

@@ -14,7 +14,8 @@ sequence. Pages may be stored head by head: then pass the transposed view.
                                             parents.flatten())
 
 Calls are enqueued on the stream that was current when the Ops was made, and
-refuse to run while another is. Arguments that do not fit raise ValueError
+refuse to run while another is. Threads may share an Ops: their calls are
+enqueued one after another. Arguments that do not fit raise ValueError
 before anything is enqueued, what the library refuses raises LrrtError.
 """
 from __future__ import annotations
@@ -94,10 +95,7 @@ class Ops:
         """Workspace and counters for later calls, so that none of them has to
         grow them, which a call that is captured cannot (lro_context_create
         says what calls need)."""
-        N.check(N.operators().lro_context_reserve(self.handle, workspace_bytes),
-                "lro_context_reserve")
-        N.check(N.operators().lro_context_reserve_counters(self.handle, counters),
-                "lro_context_reserve_counters")
+        _binding.reserve(self._ops, workspace_bytes, counters)
 
     # ---- operators -----------------------------------------------------------
     def rope_append(self, q, k, v, keys, values, table, sequences, positions, cos, sin,

@@ -114,3 +114,37 @@ def test_capture_that_would_grow(gpu, torch):
     N.check(N.runtime().lr_queue_is_capturing(Runtime.open_device(0), queue, C.byref(capturing)),
             "lr_queue_is_capturing")
     assert capturing.value == 0
+
+
+def test_threads_share_operators(gpu, torch):
+    """Threads that call one Ops on its stream, with sizes that outgrow its
+    workspace and its counters on the way: each gets what it gets alone."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from lrrt_b200 import ops as module
+    cases = [Attention(torch, kind, [9000, 5, 777], 16, 2, 64, 32, seed=53)
+             for kind in ("f32", "bf16", "f16")]
+    logits = torch.randn(2, 4, 30000, device="cuda")
+    scores = torch.zeros(2, 4, device="cuda")
+
+    def attend(case):
+        return lambda ops: ops.paged_attention(case.q, case.keys, case.values, case.table, case.n)
+
+    calls = [attend(case) for case in cases]
+    calls += [lambda ops: ops.beam_select(logits, scores, 4),
+              lambda ops: (attend_many(torch, ops, 3000)(),),
+              lambda ops: (attend_many(torch, ops, 7000)(),),
+              lambda ops: (compact_many(torch, ops, 500000),),
+              lambda ops: (ops.reserve(1 << 24, 70000),)]
+    with module.Ops(0) as ops:
+        want = [call(ops) for call in calls]
+        torch.cuda.synchronize()
+    with module.Ops(0) as ops, ThreadPoolExecutor(len(calls)) as pool:
+        def run(i):
+            return [[t if t is None else t.clone() for t in calls[i](ops)] for _ in range(15)]
+
+        for got, expected in zip(pool.map(run, range(len(calls))), want):
+            for each in got:
+                assert all(a is b or torch.equal(a, b) for a, b in zip(each, expected))
+    with pytest.raises(ValueError, match="closed"):
+        ops.reserve(1)
