@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include "lrrt_ops.h"
@@ -81,7 +82,8 @@ const at::Tensor &tensor_of(PyObject *object, const char *name) {
   return THPVariable_Unpack(object);
 }
 
-// A tensor on the operators' device with contiguous last dimension.
+// A tensor on the operators' device with contiguous last dimension. The operators
+// have no backward pass: a graph would end at them without a word.
 void check(const Ops &ops, const at::Tensor &t, const char *name, int64_t dims,
            at::ScalarType type) {
   if (!t.is_cuda() || t.get_device() != ops.device) {
@@ -89,6 +91,10 @@ void check(const Ops &ops, const at::Tensor &t, const char *name, int64_t dims,
   }
   if (t.scalar_type() != type) {
     refuse(name, " is ", t.scalar_type(), ", not ", type);
+  }
+  if (t.requires_grad() && at::GradMode::is_enabled()) {
+    refuse(name, " requires gradients, which these operators do not have: detach it, or call them "
+                 "under torch.no_grad()");
   }
   if (t.dim() != dims) {
     refuse(name, " has ", t.dim(), " dimensions, not ", dims);

@@ -15,7 +15,8 @@ sequence. Pages may be stored head by head: then pass the transposed view.
 
 Calls are enqueued on the stream that was current when the Ops was made, and
 refuse to run while another is. Threads may share an Ops: their calls are
-enqueued one after another. Arguments that do not fit raise ValueError
+enqueued one after another. There is no backward pass: tensors that require
+gradients are refused where these are recorded. Arguments that do not fit raise ValueError
 before anything is enqueued, what the library refuses raises LrrtError.
 """
 from __future__ import annotations
