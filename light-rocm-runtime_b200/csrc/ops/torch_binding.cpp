@@ -8,6 +8,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include "lrrt_ops.h"
@@ -66,10 +67,12 @@ void check(lr_status_t status, const char *operation) {
 }
 
 // One call of the library. It enqueues and returns, and the interpreter's lock is
-// kept meanwhile: a context serves one thread at a time.
+// kept meanwhile: a context serves one thread at a time. The library makes its device
+// current; the caller's is put back.
 template <typename Arguments>
 void call_library(lr_status_t (*function)(lro_context_t *, const Arguments *), const Ops &ops,
                   const Arguments &arguments, const char *operation) {
+  const c10::cuda::CUDAGuard guard(ops.device);
   check(function(ops.context, &arguments), operation);
 }
 
@@ -485,6 +488,7 @@ PyObject *reserve_ops(PyObject *, PyObject *arguments) {
     return nullptr;
   }
   try {
+    const c10::cuda::CUDAGuard guard(ops->device);
     check(lro_context_reserve(ops->context, bytes), "lro_context_reserve");
     check(lro_context_reserve_counters(ops->context, counters), "lro_context_reserve_counters");
   } catch (const Raised &) {

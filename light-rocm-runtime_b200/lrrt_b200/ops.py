@@ -64,8 +64,12 @@ class Ops:
 
     def __init__(self, device_index: int = 0):
         self.handle = self.queue = None
-        device = Runtime.open_device(device_index)
         self.device = torch.device("cuda", device_index)
+        with torch.cuda.device(self.device):  # the library makes its device current
+            self._open(device_index)
+
+    def _open(self, device_index: int) -> None:
+        device = Runtime.open_device(device_index)
         self.stream = torch.cuda.current_stream(self.device)
         queue, handle = C.c_void_p(), C.c_void_p()
         N.check(N.runtime().lr_queue_wrap_stream(device, self.stream.cuda_stream,
@@ -78,6 +82,10 @@ class Ops:
         self._ops = _binding.open(handle.value, device_index, N.check)
 
     def close(self) -> None:
+        with torch.cuda.device(self.device):
+            self._close()
+
+    def _close(self) -> None:
         if self.handle:
             _binding.close(self._ops)
             N.check(N.operators().lro_context_destroy(self.handle), "lro_context_destroy")

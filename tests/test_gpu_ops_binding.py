@@ -33,3 +33,23 @@ def test_gradients_are_refused(ops, torch):
         with torch.no_grad():
             call()
     assert not attend()[0].requires_grad
+
+
+def test_the_current_device_stays(gpu, torch):
+    """Operators of one device, made and called while another is current."""
+    from lrrt_b200 import ops as module
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    logits = torch.randn(1, 2, 500, device="cuda:1")
+    scores = torch.zeros(1, 2, device="cuda:1")
+    with torch.cuda.device(0):
+        with module.Ops(1) as second:
+            assert torch.cuda.current_device() == 0
+            first = second.beam_select(logits, scores, 2)
+            assert torch.cuda.current_device() == 0
+            second.reserve(1 << 26, 100000)
+            assert torch.cuda.current_device() == 0
+            again = second.beam_select(logits, scores, 2)
+        assert torch.cuda.current_device() == 0
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+        assert torch.zeros(1, device="cuda").device.index == 0
