@@ -102,7 +102,8 @@ LRRT_API lr_status_t lro_rope_tables(uint32_t positions, uint32_t rotary_dim, do
  * (2 i, 2 i + 1) when interleaved. The arithmetic is in 32 bits, rounded once.
  * A token with a sequence or a position out of range of the table or of the
  * cos/sin tables, or with no page, is padding: its queries become zeros and
- * nothing is appended. Two tokens of one call must not share a cache row.
+ * nothing is appended. Two tokens of one call must not share a cache row, nor two
+ * rows of the cache or of q_out memory.
  */
 typedef struct lro_rope_append_t {
   lro_rows_t q, q_out, k, v;
@@ -129,6 +130,7 @@ LRRT_API lr_status_t lro_rope_append(lro_context_t *context, const lro_rope_appe
  * An infinite value makes its column infinite (NaN with both signs); a NaN, or
  * a score of infinity, leaves NaN in out and lse. Sums are held in 32 bits;
  * 32-bit products are three TF32 products (about 2^-21 per product).
+ * out may be q, and must not lie partly in it, nor may its rows share memory.
  * head_dim: a multiple of 8, at most 256 (128 in 32 bits). Cache pointers and
  * strides: multiples of 16 bytes.
  */

@@ -8,7 +8,9 @@
 #include "lrrt/ops/kernels.hpp"
 
 #include <algorithm>
+#include <array>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <optional>
 #include <stdexcept>
@@ -118,6 +120,55 @@ Table table_of(const lro_table_t &table) {
 
 void check_rows(const lro_rows_t &rows, size_t bytes, const char *text) {
   require(rows.data != nullptr && multiple_of(rows.data, bytes), text);
+}
+
+// Refuses places of `width` neighbouring elements that are written to, `sizes` of
+// them `strides` apart, unless each stride spans all that lies within it: others
+// may share memory.
+template <size_t N>
+void require_apart(std::array<int64_t, N> strides, std::array<uint64_t, N> sizes, uint64_t width,
+                   const char *text) {
+  std::array<std::pair<uint64_t, uint64_t>, N> axes;
+  for (size_t i = 0; i < N; ++i) {
+    axes[i] = {static_cast<uint64_t>(std::abs(int64_t{stride_of(strides[i])})), sizes[i]};
+    if (sizes[i] == 0) {
+      return;
+    }
+  }
+  std::sort(axes.begin(), axes.end());
+  for (const auto &[stride, size] : axes) {
+    if (size > 1u) {
+      require(stride >= width, text);
+      width += stride * (size - 1u);
+    }
+  }
+}
+
+// Whether a new table's rows share memory with the table's: of the same stride
+// each two of them that come near, else the extents of all.
+bool tables_meet(const int32_t *out, int64_t out_stride, uint32_t out_rows,
+                 const lro_table_t &table) {
+  if (out_rows == 0 || table.rows == 0 || table.columns == 0) {
+    return false;
+  }
+  const int64_t distance =
+      reinterpret_cast<intptr_t>(table.pages) - reinterpret_cast<intptr_t>(out);
+  const int64_t width = int64_t{table.columns} * 4, stride = 4 * table.row_stride;
+  const int64_t out_last = 4 * out_stride * (int64_t{out_rows} - 1);
+  const int64_t last = stride * (int64_t{table.rows} - 1);
+  if (out_stride == table.row_stride && stride != 0) {
+    // Row i of the table is `distance` + stride (i - j) past row j of the new one.
+    const int64_t nearest = -distance / stride;
+    for (int64_t k = nearest - 1; k <= nearest + 1; ++k) {
+      if (k > -int64_t{out_rows} && k < int64_t{table.rows} &&
+          std::abs(distance + stride * k) < width) {
+        return true;
+      }
+    }
+    return false;
+  }
+  return distance + std::min<int64_t>(last, 0) < std::max<int64_t>(out_last, 0) + width &&
+         distance + std::max<int64_t>(last, 0) + width > std::min<int64_t>(out_last, 0);
 }
 
 // Whether vectors of `bytes` bytes fit rows of this layout.
@@ -240,6 +291,17 @@ void rope_append(lro_context_t &context, const lro_rope_append_t &a) {
   check_rows(a.k, element, "k is missing or misaligned");
   check_rows(a.v, element, "v is missing or misaligned");
   require(cache_takes(a.cache, element), "the cache is misaligned");
+  require_apart(std::array{a.q_out.row_stride, a.q_out.head_stride},
+                std::array{uint64_t{a.tokens}, uint64_t{a.heads}}, dim,
+                "rows of q_out share memory");
+  const std::array cache_sizes{uint64_t{a.cache.page_count}, uint64_t{a.cache.page_size},
+                               uint64_t{a.cache.kv_heads}};
+  require_apart(std::array{a.cache.key_page_stride, a.cache.key_token_stride,
+                           a.cache.key_head_stride},
+                cache_sizes, dim, "rows of keys share memory");
+  require_apart(std::array{a.cache.value_page_stride, a.cache.value_token_stride,
+                           a.cache.value_head_stride},
+                cache_sizes, dim, "rows of values share memory");
 
   // The widest vector that all rows and columns are made of: 16 bytes, 8 (for
   // 16-bit rows such as a half of 20 elements), or single elements. Measured with
@@ -320,6 +382,9 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
   require(a.lengths != nullptr, "lengths are missing");
   check_rows(a.q, element, "q is missing or misaligned");
   check_rows(a.out, element, "out is missing or misaligned");
+  require_apart(std::array{a.out.row_stride, a.out.head_stride},
+                std::array{uint64_t{a.table.rows}, uint64_t{a.heads}}, a.cache.head_dim,
+                "rows of out share memory");
   require(cache_takes(a.cache, 16),
           "cache pointers and strides must be multiples of 16 bytes");
 
@@ -461,8 +526,10 @@ void pages_fork(lro_context_t &context, const lro_pages_fork_t &a) {
   require(a.rows_out <= 0x7fffffffu &&
               uint64_t{a.rows_out} * (uint64_t{a.table.columns} + 1u) < (uint64_t{1} << 32),
           "the new table is too large");
-  require(a.rows_out == 0 || a.table.columns == 0 || a.table_out != a.table.pages,
-          "table_out must not be the table");
+  require(!tables_meet(a.table_out, a.table_out_row_stride, a.rows_out, a.table),
+          "table_out must not be the table, nor share memory with it");
+  require_apart(std::array{a.table_out_row_stride}, std::array{uint64_t{a.rows_out}},
+                a.table.columns, "rows of table_out share memory");
   const size_t rows = a.rows_out, pages = a.pool.page_count;
   PlanArrays arrays{};
   PageMove *list = nullptr;
@@ -501,8 +568,11 @@ void pages_compact(lro_context_t &context, const lro_pages_compact_t &a) {
   require(a.status != nullptr, "status is missing");
   require(a.table_out != nullptr || a.table.rows == 0 || a.table.columns == 0,
           "table_out is missing");
-  require(a.table_out != a.table.pages || a.table_out_row_stride == a.table.row_stride,
-          "table_out is the table, with another stride");
+  require((a.table_out == a.table.pages && a.table_out_row_stride == a.table.row_stride) ||
+              !tables_meet(a.table_out, a.table_out_row_stride, a.table.rows, a.table),
+          "table_out shares memory with the table and is not it");
+  require_apart(std::array{a.table_out_row_stride}, std::array{uint64_t{a.table.rows}},
+                a.table.columns, "rows of table_out share memory");
   const size_t pages = a.pool.page_count;
   PlanArrays arrays{};
   PageMove *list = nullptr;

@@ -7,6 +7,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -136,6 +137,14 @@ lro_rows_t rows_of(const Ops &ops, const at::Tensor &t, const char *name,
            "]");
   }
   return {t.data_ptr(), t.stride(0), t.stride(1)};
+}
+
+// Where an output may be the input as it is, but not lie partly in it.
+void check_apart(const at::Tensor &out, const char *name, const at::Tensor &in,
+                 const char *in_name) {
+  if (at::get_overlap_status(out, in) == at::MemOverlapStatus::Partial) {
+    refuse(name, " lies partly in ", in_name);
+  }
 }
 
 uint32_t type_of(const at::Tensor &t, const char *what) {
@@ -288,6 +297,9 @@ PyObject *rope_append(const Ops &ops, PyObject *const *a) {
   at::Tensor out = a[12] != Py_None ? tensor_of(a[12], "out")
                                     : empty(ops, {tokens, heads, dim}, type);
   call.q_out = rows_of(ops, out, "out", {tokens, heads, dim}, type);
+  check_apart(out, "out", q, "q");
+  check_apart(out, "out", tensor_of(a[2], "k"), "k");
+  check_apart(out, "out", tensor_of(a[3], "v"), "v");
   call_library(lro_rope_append, ops, call, "lro_rope_append");
   return wrap(std::move(out));
 }
@@ -317,6 +329,7 @@ PyObject *paged_attention(const Ops &ops, PyObject *const *a) {
   at::Tensor out = a[10] != Py_None ? tensor_of(a[10], "out")
                                     : empty(ops, {rows, heads, dim}, type);
   call.out = rows_of(ops, out, "out", {rows, heads, dim}, type);
+  check_apart(out, "out", q, "q");
   at::Tensor lse = empty(ops, {rows, heads}, at::kFloat);
   call.lse = static_cast<float *>(lse.data_ptr());
   call_library(lro_paged_attention, ops, call, "lro_paged_attention");
