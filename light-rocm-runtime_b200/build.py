@@ -8,6 +8,7 @@ Outputs (git-ignored, shipped with the working tree):
   lib/decoder_ops.cubin + .json   per-operation decode kernels as an lrrt::bundle
   lib/liblrrt_ops.so              paged-cache operators (include/lrrt_ops.h)
   lib/lrrt_ops_torch.so           the same on torch tensors, a Python extension
+                                  (where torch is installed)
   lib/paged_ops.cubin             their sm_100a kernels
   _build/tests/stateful_graph_fixture.cubin  sm_100a scheduler fixture kernels (tests)
   _build/tests/*                  C++ host tests (tests/cpp)
@@ -16,6 +17,7 @@ Rebuilds a target only when one of its inputs is newer than it.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -112,14 +114,18 @@ def build(verbose: bool = False) -> dict[str, Path]:
               "-lrt", "-ldl", "-lpthread", "-Wl,-rpath,$ORIGIN"], verbose)
     outputs["driver"] = driver
 
-    # The operators on torch tensors (lrrt_b200/ops.py): a Python extension.
+    # The operators on torch tensors (lrrt_b200/ops.py): a Python extension, and the
+    # one part that needs torch. Without it the rest is built all the same.
     binding = LIB / "lrrt_ops_torch.so"
     binding_source = csrc / "ops" / "torch_binding.cpp"
-    if _stale(binding, [binding_source] + headers + [ops]):
-        _run([CXX, *CXXFLAGS, *_torch_flags(), "-shared", "-fvisibility=hidden",
-              str(binding_source), "-o", str(binding), f"-L{LIB}", "-llrrt_ops", "-llrrt",
-              *_torch_libraries(), "-Wl,-rpath,$ORIGIN"], verbose)
-    outputs["ops_torch"] = binding
+    if importlib.util.find_spec("torch") is None:
+        print(f"torch is not installed: {binding.name} is left out")
+    else:
+        if _stale(binding, [binding_source] + headers + [ops]):
+            _run([CXX, *CXXFLAGS, *_torch_flags(), "-shared", "-fvisibility=hidden",
+                  str(binding_source), "-o", str(binding), f"-L{LIB}", "-llrrt_ops", "-llrrt",
+                  *_torch_libraries(), "-Wl,-rpath,$ORIGIN"], verbose)
+        outputs["ops_torch"] = binding
 
     for name in ("qwen_stateful_graph", "qwen_prefill", "decoder_ops", "paged_ops"):
         source = csrc / "kernels" / f"{name}.cu"
