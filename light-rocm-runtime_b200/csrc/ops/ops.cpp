@@ -25,10 +25,14 @@ using namespace lrrt::ops;
 
 thread_local std::string t_last_error;
 
-void set_error(const std::string &text) noexcept {
+// The text of an error, or none where there is no memory for it.
+template <typename... Parts> void set_error(const Parts &...parts) noexcept {
   try {
-    t_last_error = text;
+    std::string text;
+    (text.append(parts), ...);
+    t_last_error = std::move(text);
   } catch (...) {
+    t_last_error.clear();
   }
 }
 
@@ -39,17 +43,17 @@ template <typename Body> lr_status_t guarded(const char *what, Body body) noexce
   } catch (const lrrt::Error &error) {
     char detail[512] = {};
     lr_last_error_detail(detail, sizeof(detail));
-    set_error(std::string(what) + ": " + error.what() +
-              (detail[0] != '\0' ? std::string(" [") + detail + "]" : std::string()));
+    const bool more = detail[0] != '\0';
+    set_error(what, ": ", error.what(), more ? " [" : "", detail, more ? "]" : "");
     return error.status();
   } catch (const std::invalid_argument &error) {
-    set_error(std::string(what) + ": " + error.what());
+    set_error(what, ": ", error.what());
     return LR_ERROR_INVALID_ARGUMENT;
   } catch (const std::exception &error) {
-    set_error(std::string(what) + ": " + error.what());
+    set_error(what, ": ", error.what());
     return LR_ERROR_RUNTIME;
   } catch (...) {
-    set_error(std::string(what) + ": unknown failure");
+    set_error(what, ": unknown failure");
     return LR_ERROR_RUNTIME;
   }
 }

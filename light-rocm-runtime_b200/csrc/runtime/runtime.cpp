@@ -26,6 +26,7 @@
 #include <cstring>
 #include <memory>
 #include <mutex>
+#include <new>
 #include <string>
 #include <unordered_map>
 #include <unordered_set>
@@ -677,10 +678,14 @@ LRRT_API lr_status_t lr_queue_wrap_stream(lr_device_t device, void *stream,
   if (open_device_state(device.index) == nullptr || queue == nullptr) {
     return LR_ERROR_INVALID_ARGUMENT;
   }
-  lr_queue_t *created =
-      new lr_queue_t{device.index, static_cast<CUstream>(stream), true};
-  g_queues.insert(created);
-  *queue = created;
+  try {
+    std::unique_ptr<lr_queue_t> created(
+        new lr_queue_t{device.index, static_cast<CUstream>(stream), true});
+    g_queues.insert(created.get());
+    *queue = created.release();
+  } catch (const std::bad_alloc &) {
+    return LR_ERROR_RUNTIME;
+  }
   return LR_SUCCESS;
 }
 
