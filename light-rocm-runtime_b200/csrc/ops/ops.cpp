@@ -134,7 +134,7 @@ void require_apart(std::array<int64_t, N> strides, std::array<uint64_t, N> sizes
                    const char *text) {
   std::array<std::pair<uint64_t, uint64_t>, N> axes;
   for (size_t i = 0; i < N; ++i) {
-    axes[i] = {static_cast<uint64_t>(std::abs(int64_t{stride_of(strides[i])})), sizes[i]};
+    axes[i] = {static_cast<uint64_t>(std::abs(strides[i])), sizes[i]};
     if (sizes[i] == 0) {
       return;
     }
@@ -463,6 +463,9 @@ bool pool_moves(const lro_pool_t &pool, MoveArgs &args) {
            multiple_of(pool.page_stride_bytes, 1, bytes) && pool.row_bytes % bytes == 0;
   };
   require(fits(4), "pool pointers, strides and row_bytes must be multiples of 4 bytes");
+  require_apart(std::array{pool.layer_stride_bytes, pool.page_stride_bytes},
+                std::array{uint64_t{pool.layers}, uint64_t{pool.page_count}}, run * pool.segments,
+                "the pool's pages share memory");
   const bool wide = fits(16); // 4 bytes at a time: 86 us where 16 take 78
   const uint64_t slices = ceil_div(run, kMoveSliceVectors * (wide ? 16u : 4u));
   const uint64_t units = uint64_t{pool.layers} * 2u * pool.segments * slices;

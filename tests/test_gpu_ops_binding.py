@@ -127,3 +127,26 @@ def test_outputs_beside_inputs(ops, torch):
     assert got[:, 0].tolist() == [0, 1, 2, 3] and (got[:, 1:] == -1).all()
     got, _ = ops.compact_pages(*pools, table[:, 5:], table_out=table[:, 5:])
     assert got[:, 0].tolist() == [0, 1, 2, 3]
+
+
+def test_pools_whose_pages_share_memory_are_refused(ops, torch):
+    """Expanded layers or pages; pages of one layer, and pages woven with others'
+    by layer, are as they were."""
+    one = torch.randn(2, 8, 4, 2, 8, device="cuda")
+    table = torch.tensor([[7, 2], [5, -1]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([8, 3], dtype=torch.int32, device="cuda")
+    both = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+    for pool in (one[:1].expand(2, 8, 4, 2, 8), one[:, :1].expand(2, 8, 4, 2, 8)):
+        for call in (lambda p: ops.fork_pages(p, p, table, lengths, both),
+                     lambda p: ops.compact_pages(p, p, table),
+                     lambda p: ops.copy_pages(p, p, both, both + 2)):
+            with pytest.raises(N.LrrtError, match="share memory"):
+                call(pool)
+    woven = lambda x: x.transpose(0, 1).contiguous().transpose(0, 1)  # noqa: E731
+    for view in (torch.clone, woven, lambda x: woven(x)[:, ::2], lambda x: x.clone()[:, :, :2],
+                 lambda x: x[:1].clone()):  # woven: [pages][layers] in memory
+        keys, values = view(one), view(one)
+        want = keys.clone()
+        want[:, 2:4] = keys[:, :2]
+        ops.copy_pages(keys, values, both, both + 2)
+        assert torch.equal(keys, want) and torch.equal(values, want)
