@@ -118,21 +118,24 @@ __device__ __forceinline__ void split_tf32(uint32_t bits, uint32_t &high, uint32
 // Weights and values are split so that infinite values go through: both parts of
 // a weight are positive, so that an infinity times them is that infinity (0, and a
 // negative rest, would make a NaN of it), and the second part of an infinite value
-// is finite. Weights and values are cut off after their first part, not rounded:
-// the rest has their sign, and NaN stays NaN.
+// is finite. Weights and values are cut off after their first part, not rounded: the
+// rest has their sign, and NaN stays NaN. The rest is rounded to nearest.
+__device__ __forceinline__ uint32_t rounded_tf32(float x) {
+  return (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+}
 
 // A weight as two TF32 numbers; 2^-126 is nothing beside any sum.
 __device__ __forceinline__ void split_weight_tf32(uint32_t bits, uint32_t &high, uint32_t &low) {
   high = bits & 0xffffe000u;
-  low = __float_as_uint(fmaxf(__uint_as_float(bits) - __uint_as_float(high), 0x1p-126f));
+  low = rounded_tf32(fmaxf(__uint_as_float(bits) - __uint_as_float(high), 0x1p-126f));
 }
 
-// A value: the rest is below 2^-10 of the largest number. That of an infinity is
-// a NaN before the minimum.
+// A value: the rest is below 2^117, and stays below it where it is rounded, so that the
+// largest number does not become an infinity. That of an infinity is a NaN before
+// the minimum.
 __device__ __forceinline__ void split_value_tf32(uint32_t bits, uint32_t &high, uint32_t &low) {
   high = bits & 0xffffe000u;
-  const float rest = __uint_as_float(bits) - __uint_as_float(high);
-  low = __float_as_uint(fminf(rest, 0x1p118f)) & 0xffffe000u;
+  low = rounded_tf32(fminf(__uint_as_float(bits) - __uint_as_float(high), 0x1.ffcp116f));
 }
 
 // Two weights as a pair of 16-bit numbers, and what they leave over as another. In
