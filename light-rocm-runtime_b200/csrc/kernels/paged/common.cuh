@@ -45,9 +45,6 @@ template <typename T> struct Words;
 template <> struct Words<float> {
   static constexpr uint32_t kLeast = 0xff800000u; // -infinity
   static __device__ __forceinline__ uint32_t of(float x, float) { return __float_as_uint(x); }
-  static __device__ __forceinline__ void set(uint32_t &word, int, float x) {
-    word = __float_as_uint(x);
-  }
   static __device__ __forceinline__ float value(uint32_t word, int) {
     return __uint_as_float(word);
   }
@@ -63,11 +60,6 @@ template <> struct Words<__nv_bfloat16> {
     uint32_t word;
     memcpy(&word, &pair, 4);
     return word;
-  }
-  static __device__ __forceinline__ void set(uint32_t &word, int half, __nv_bfloat16 x) {
-    uint16_t bits;
-    memcpy(&bits, &x, 2);
-    word = half == 0 ? (word & 0xffff0000u) | bits : (word & 0xffffu) | uint32_t{bits} << 16;
   }
   static __device__ __forceinline__ float value(uint32_t word, int half) {
     return __uint_as_float(half == 0 ? word << 16 : word & 0xffff0000u);
@@ -91,11 +83,6 @@ template <> struct Words<__half> {
     uint32_t word;
     memcpy(&word, &pair, 4);
     return word;
-  }
-  static __device__ __forceinline__ void set(uint32_t &word, int half, __half x) {
-    uint16_t bits;
-    memcpy(&bits, &x, 2);
-    word = half == 0 ? (word & 0xffff0000u) | bits : (word & 0xffffu) | uint32_t{bits} << 16;
   }
   static __device__ __forceinline__ float value(uint32_t word, int half) {
     __half2 x;
