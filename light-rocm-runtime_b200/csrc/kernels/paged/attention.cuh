@@ -13,8 +13,10 @@
 //  - The query heads of one key-value head share each row that is read: scores
 //    are computed transposed, S^T = K Q^T, with 16 keys as the rows of the
 //    matrix product and 8 query heads as its columns, and so are the outputs,
-//    O^T = V^T P^T. One query row per head leaves nothing to fill the 128 rows
-//    of a tcgen05 tile from the query side; these shapes (m16n8) waste none.
+//    O^T = V^T P^T. These shapes (m16n8) waste nothing of up to 8 heads, which
+//    memory bounds. (A tcgen05 tile of 128 keys by 16 heads is not built; groups
+//    of 9 to 16 heads, which issue slots bound, would be the ones to gain.) A
+//    tile's products are summed by themselves and added in rounded 32 bits.
 //    16-bit weights are split into two 16-bit parts, so that the probabilities
 //    keep 16 bits (in f16 down to 2^-39 of a row's largest); 32-bit operands into
 //    two TF32 parts (three products).
@@ -27,11 +29,12 @@
 //    timing.
 //
 // Measured (cache reads at 6.5 TB/s take the time in brackets): 64 ragged
-// sequences of up to 8192 keys, 32 heads over 8 of 128 elements in bf16, 135 us
-// (122); two of about 123000 keys with capped scores 49 us (38); pages of one token
-// 165 us. Few keys are bound by latency (launch, lengths, page numbers, first
-// tile, joining): 32 sequences of 1152, 14 heads over 2 of 64 in f32, 16.2 us
-// (5.5); one of 160, 7.8 us.
+// sequences of up to 8192 keys, 32 heads over 8 of 128 elements in bf16, 136 us
+// (122), in pages of one token 162 us (133); two of about 123000 keys with capped
+// scores 50 us (38); 128 heads over 8 in bf16 132 us (109), 16 over 4 of 128 in f32
+// 175 us (132). Few keys are bound by latency (launch, lengths, page numbers, first
+// tile, joining): 32 sequences of 1152, 14 heads over 2 of 64 in f32, 15.9 us
+// (5.5); one of 160, 7.7 us.
 #ifndef LRRT_PAGED_ATTENTION_CUH_
 #define LRRT_PAGED_ATTENTION_CUH_
 
@@ -196,10 +199,12 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
   static constexpr uint32_t kChunks = kRowBytes / 16u; // 16-byte chunks of a row
   static constexpr uint32_t kRowsPerPass = 32u / kChunks;
   static constexpr uint32_t kPasses = kKeys / kRowsPerPass / Team; // of one warp
-  // Passes at once for tiles of several pages: all for large tiles (8 keys a
-  // page, f32: 114 us, 125 with four), four where that code is in the way of the
-  // rest (128 heads over 8, one page: 130 us instead of 134; teams of 16-bit
-  // elements 139 instead of 151).
+  // Passes at once for tiles of several pages: all for large tiles (pages of 8
+  // keys, 64 ragged sequences of up to 8192: f32 of 128, 16 heads over 4, 170 us,
+  // 175 with four; of 96, 48 over 4, 183 and 195; bf16 of 256, 32 over 4, 164 and
+  // 168), four where that code is in the way of the rest (pages of 64: bf16 of 128,
+  // 128 over 8, 131 us instead of 133; of 256, 64 over 4, 146 instead of 149). Of the
+  // large tiles f32 teams of 128 alone lose by it, 253 and 236 us.
   static constexpr int kScatteredPasses = kRowBytes > 256u && (kWide || Team == 1) ? 16 : 4;
   static constexpr uint32_t kKeyTiles = kKeys / 16u;
   static constexpr uint32_t kSteps = Dim * sizeof(T) / 32u; // of Q K^T (32 bytes of a row)

@@ -14,8 +14,9 @@
 // for the two rows of 151936 that the fullest SM has of 256), and by the fixed
 // work of a part (7 us to the end of the launch: floor, second reading, ranking,
 // joining) where there are few rows. Measured: 256 rows of 151936 logits in bf16,
-// 8 beams a group, 16 wanted, 24.3 us (3.2 TB/s; with two rounds under way in
-// registers 30.8 us); 200 rows in f32 29.3 us (4.2 TB/s); 4 rows in f32, 9.4 us.
+// 8 beams a group, 16 wanted, 23.6 us (3.3 TB/s; an earlier form with two rounds under
+// way in registers 30.8 us, with the ring 24.3); 200 rows in f32 27.6 us (4.4 TB/s);
+// 4 rows in f32, 9.9 us.
 //
 // Pooled elements are 64-bit keys, the value's order in the upper half and the
 // complement of the index in the lower, so that no two are equal and the order

@@ -394,8 +394,8 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
 
   // The next of the kernels' widths: what lies past the head's elements are
   // products of zeros. Heads of 96 in f32 (8 over 1, 6 sequences of about 90000
-  // keys) as 96 and as 128 elements: 98 and 115 us; of 80 in f16 (128 over 8, 8
-  // sequences of 3900): 35 and 38 us.
+  // keys) as 96 and as 128 elements: 95 and 112 us; of 80 in f16 (128 over 8, 8
+  // sequences of 3900): 28 and 31 us.
   uint32_t dim = 256;
   for (const uint32_t width : {128u, 96u, 64u}) {
     dim = a.cache.head_dim <= width ? width : dim;
@@ -403,9 +403,9 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
   const uint32_t group = a.heads / a.cache.kv_heads;
   // Up to 16 query heads share a row that is read; blocks of them read it one
   // after another. Measured (64 ragged sequences of up to 8192 keys), blocks of 16
-  // heads and of 8: bf16, 128 heads over 8, of 128 elements 128 and 226 us, of 64 86
-  // and 156 us; 64 over 4 of 256 139 and 239 us; f32, 128 over 8 of 64 178 and 226 us,
-  // 48 over 4 of 128 249 and 318 us.
+  // heads and of 8: bf16, 128 heads over 8, of 128 elements 132 and 228 us, of 64 85
+  // and 158 us; 64 over 4 of 256 145 and 241 us; f32, 128 over 8 of 64 172 and 221 us,
+  // 48 over 4 of 128 254 and 320 us.
   const uint32_t heads = group > 8u ? 16u : 8u;
   PagedAttentionArgs args{};
   args.q = rows_of(a.q);
@@ -640,9 +640,9 @@ void beam_select(lro_context_t &context, const lro_beam_select_t &a) {
   // ones where it has its SM alone, 0.7 and 0.48 us where two share it; a part's
   // fixed work (floor, ranking) 4.2 us alone and 4.8 us beside another; joining
   // a row's parts 2.5 us and a little for each. Measured, 151936 logits: 256 rows in
-  // bf16 1, 2, 3 parts 25, 33, 38 us; 96 rows in f32 1, 2, 3, 4 parts 21, 21, 20.7,
-  // 27 us; 32 rows in bf16 1, 2, 4, 5, 8 parts 17, 15, 13, 14.5, 13.6 us; 4 rows in
-  // f32 4, 8, 20, 38 parts 11.4, 10.0, 9.4, 10.7 us.
+  // bf16 1, 2, 3 parts 24, 31, 37 us; 96 rows in f32 1, 2, 3, 4 parts 19, 19, 16.5,
+  // 20 us; 32 rows in bf16 1, 2, 4, 5, 8 parts 15, 13, 11.2, 12.4, 11.5 us; 4 rows in
+  // f32 4, 8, 20, 38 parts 11.8, 10.2, 9.9, 10.5 us.
   const uint32_t round = beam_round(static_cast<uint32_t>(element));
   const uint64_t rounds = ceil_div(a.vocab, round);
   const uint64_t most = std::min<uint64_t>({rounds, kBeamMaximumParts, kBeamPool / a.count});
