@@ -297,9 +297,11 @@ PyObject *rope_append(const Ops &ops, PyObject *const *a) {
   at::Tensor out = a[12] != Py_None ? tensor_of(a[12], "out")
                                     : empty(ops, {tokens, heads, dim}, type);
   call.q_out = rows_of(ops, out, "out", {tokens, heads, dim}, type);
-  check_apart(out, "out", q, "q");
-  check_apart(out, "out", tensor_of(a[2], "k"), "k");
-  check_apart(out, "out", tensor_of(a[3], "v"), "v");
+  if (a[12] != Py_None) {
+    check_apart(out, "out", q, "q");
+    check_apart(out, "out", tensor_of(a[2], "k"), "k");
+    check_apart(out, "out", tensor_of(a[3], "v"), "v");
+  }
   call_library(lro_rope_append, ops, call, "lro_rope_append");
   return wrap(std::move(out));
 }
@@ -329,7 +331,9 @@ PyObject *paged_attention(const Ops &ops, PyObject *const *a) {
   at::Tensor out = a[10] != Py_None ? tensor_of(a[10], "out")
                                     : empty(ops, {rows, heads, dim}, type);
   call.out = rows_of(ops, out, "out", {rows, heads, dim}, type);
-  check_apart(out, "out", q, "q");
+  if (a[10] != Py_None) {
+    check_apart(out, "out", q, "q");
+  }
   at::Tensor lse = empty(ops, {rows, heads}, at::kFloat);
   call.lse = static_cast<float *>(lse.data_ptr());
   call_library(lro_paged_attention, ops, call, "lro_paged_attention");
