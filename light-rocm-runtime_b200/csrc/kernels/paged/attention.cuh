@@ -133,12 +133,13 @@ __device__ __forceinline__ void split_weight_tf32(uint32_t bits, uint32_t &high,
   low = rounded_tf32(fmaxf(__uint_as_float(bits) - __uint_as_float(high), 0x1p-126f));
 }
 
-// A value: the rest is below 2^117, and stays below it where it is rounded, so that the
-// largest number does not become an infinity. That of an infinity is a NaN before
-// the minimum.
+// A value: the rest's size is below 2^117, and stays below it where it is rounded, so
+// that the largest numbers do not become infinities. That of an infinity is a NaN
+// before the minimum.
 __device__ __forceinline__ void split_value_tf32(uint32_t bits, uint32_t &high, uint32_t &low) {
   high = bits & 0xffffe000u;
-  low = rounded_tf32(fminf(__uint_as_float(bits) - __uint_as_float(high), 0x1.ffcp116f));
+  const float rest = __uint_as_float(bits) - __uint_as_float(high);
+  low = rounded_tf32(fmaxf(fminf(rest, 0x1.ffcp116f), -0x1.ffcp116f));
 }
 
 // Two weights as a pair of 16-bit numbers, and what they leave over as another. In

@@ -267,3 +267,16 @@ def test_beam_select_any_number_of_candidates(ops, torch, beams):
         logits, scores, finished = beam_case(rng, 3, beams, 200)
         beam_check(ops, torch, "f32", logits, scores, count, finished, end_token=1)
         beam_check(ops, torch, "bf16", logits, scores, count)
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("below", [0, 1, 2 ** 10, 2 ** 12, 2 ** 13 - 1])
+def test_attention_largest_values(ops, torch, sign, below):
+    """The value of a single key at either end of 32 bits, some units in the last
+    place inside it, is the output, to 2^-20 of it."""
+    most = torch.finfo(torch.float32).max
+    case = Attention(torch, "f32", [1, 1], 8, 2, 128, 16, seed=49)
+    value = torch.tensor(most).view(torch.int32).sub(below).view(torch.float32).item() * sign
+    case.values[..., 7] = value
+    out, _ = ops.paged_attention(case.q, case.keys, case.values, case.table, case.n)
+    assert ((out[:, :, 7].double() / value - 1).abs() <= 2.0 ** -20).all()
