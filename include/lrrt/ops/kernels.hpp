@@ -95,7 +95,7 @@ struct RopeAppendArgs {
 // would not fit one warp's registers. A tile is 16 keys and values, or 32 of the
 // short rows of 128 bytes: 8 KB, and 16 KB for rows of 512 bytes. Eight units
 // have three tiles each (two beside states of 16 heads); of the large tiles six
-// have two (four with three: 207 us instead of 175 for 64 sequences of up to 8192
+// have two (four with three: 216 us instead of 180 for 64 sequences of up to 8192
 // keys, 16 heads over 4 of 128 in f32), four have three beside states of 256 elements, or
 // as teams (two beside 16 heads of 256).
 // Rows of 96 elements (for heads of 65 to 96) lie in the places of 128.

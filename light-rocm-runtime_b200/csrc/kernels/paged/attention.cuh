@@ -32,7 +32,7 @@
 // sequences of up to 8192 keys, 32 heads over 8 of 128 elements in bf16, 136 us
 // (122), in pages of one token 162 us (133); two of about 123000 keys with capped
 // scores 50 us (38); 128 heads over 8 in bf16 132 us (109), 16 over 4 of 128 in f32
-// 175 us (132). Few keys are bound by latency (launch, lengths, page numbers, first
+// 180 us (132). Few keys are bound by latency (launch, lengths, page numbers, first
 // tile, joining): 32 sequences of 1152, 14 heads over 2 of 64 in f32, 15.9 us
 // (5.5); one of 160, 7.7 us.
 #ifndef LRRT_PAGED_ATTENTION_CUH_
@@ -135,7 +135,9 @@ __device__ __forceinline__ void split_weight_tf32(uint32_t bits, uint32_t &high,
 
 // A value: the rest's size is below 2^117, and stays below it where it is rounded, so
 // that the largest numbers do not become infinities. That of an infinity is a NaN
-// before the minimum.
+// before the minimum. (Not rounded, and so not bounded from below, 171 us where this
+// takes 180, 64 ragged sequences of 16 heads over 4 of 128, and errors of 3.6e-7
+// where these are 2.5e-7.)
 __device__ __forceinline__ void split_value_tf32(uint32_t bits, uint32_t &high, uint32_t &low) {
   high = bits & 0xffffe000u;
   const float rest = __uint_as_float(bits) - __uint_as_float(high);
@@ -201,11 +203,11 @@ template <typename T, int Dim, int HeadTiles, int Team> class PagedAttention {
   static constexpr uint32_t kRowsPerPass = 32u / kChunks;
   static constexpr uint32_t kPasses = kKeys / kRowsPerPass / Team; // of one warp
   // Passes at once for tiles of several pages: all for large tiles (pages of 8
-  // keys, 64 ragged sequences of up to 8192: f32 of 128, 16 heads over 4, 170 us,
-  // 175 with four; of 96, 48 over 4, 183 and 195; bf16 of 256, 32 over 4, 164 and
+  // keys, 64 ragged sequences of up to 8192: f32 of 128, 16 heads over 4, 174 us,
+  // 178 with four; of 96, 48 over 4, 189 and 199; bf16 of 256, 32 over 4, 164 and
   // 168), four where that code is in the way of the rest (pages of 64: bf16 of 128,
   // 128 over 8, 131 us instead of 133; of 256, 64 over 4, 146 instead of 149). Of the
-  // large tiles f32 teams of 128 alone lose by it, 253 and 236 us.
+  // large tiles f32 teams of 128 alone lose by it, 258 and 245 us.
   static constexpr int kScatteredPasses = kRowBytes > 256u && (kWide || Team == 1) ? 16 : 4;
   static constexpr uint32_t kKeyTiles = kKeys / 16u;
   static constexpr uint32_t kSteps = Dim * sizeof(T) / 32u; // of Q K^T (32 bytes of a row)

@@ -394,7 +394,7 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
 
   // The next of the kernels' widths: what lies past the head's elements are
   // products of zeros. Heads of 96 in f32 (8 over 1, 6 sequences of about 90000
-  // keys) as 96 and as 128 elements: 95 and 112 us; of 80 in f16 (128 over 8, 8
+  // keys) as 96 and as 128 elements: 98 and 115 us; of 80 in f16 (128 over 8, 8
   // sequences of 3900): 28 and 31 us.
   uint32_t dim = 256;
   for (const uint32_t width : {128u, 96u, 64u}) {
@@ -404,8 +404,8 @@ void paged_attention(lro_context_t &context, const lro_paged_attention_t &a) {
   // Up to 16 query heads share a row that is read; blocks of them read it one
   // after another. Measured (64 ragged sequences of up to 8192 keys), blocks of 16
   // heads and of 8: bf16, 128 heads over 8, of 128 elements 132 and 228 us, of 64 85
-  // and 158 us; 64 over 4 of 256 145 and 241 us; f32, 128 over 8 of 64 172 and 221 us,
-  // 48 over 4 of 128 254 and 320 us.
+  // and 158 us; 64 over 4 of 256 145 and 241 us; f32, 128 over 8 of 64 175 and 238 us,
+  // 48 over 4 of 128 258 and 326 us.
   const uint32_t heads = group > 8u ? 16u : 8u;
   PagedAttentionArgs args{};
   args.q = rows_of(a.q);
